@@ -321,6 +321,50 @@ int zp_layernorm_silu_backward(int64_t rows, int width, const float *x, const fl
                                const float *dy, float *dx, float *dgamma, float *dbeta,
                                void *work, size_t work_bytes, void *stream);
 
+/* Operators over the rows of a matrix, for layers in front of, between and behind those above.
+ * `dtype`: a zp_dtype; sums and row statistics are fp32 in all of them, each result is rounded once.
+ * A matrix [rows, width] has its rows `ld*` >= width elements apart (results without an `ld` lie row
+ * behind row); any width from 1 on, any address that is a multiple of an element's size.  Weight and
+ * bias [width] are of type `param_dtype`, the rows' own or ZP_F32, and either may be NULL (1, 0).
+ * Results may not overlap inputs.
+ *
+ * Dropout: y = x / keep where the element is kept, 0 where it is not (also where x is not finite).
+ * `state` (device, two int64: seed and offset) and the element's number r * width + c decide: with
+ * i = r * width + c, the (i % 8)-th 16-bit half, low half first, of the four words that Philox-4x32-10
+ * gives for counter (i / 8, offset) under key `seed` has to be at least t = floor(65536 p + 1/2);
+ * keep = 1 - t / 65536.  Nothing is stored: the VJP is the same call on the gradient.  The state is
+ * read when the kernel runs, so a recorded graph follows what is written there between replays.   */
+typedef enum zp_dtype { ZP_F32 = 0, ZP_F16 = 1, ZP_BF16 = 2 } zp_dtype;
+int zp_dropout(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx, double p,
+               const int64_t *state, void *y, int64_t ldy, void *stream);
+
+/* Layer norm, y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps) over each row.  mean and
+ * rstd [rows] are kept for the backward (both NULL: no backward follows).  Backward: any of dx, dweight,
+ * dbias may be NULL; dweight and dbias are summed in a fixed order and need
+ * `work`: zp_rowwise_work_bytes(rows, width) bytes of device scratch, caller-owned.               */
+size_t zp_rowwise_work_bytes(int64_t rows, int64_t width);
+int zp_layernorm_forward(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx,
+                         int param_dtype, const void *weight, const void *bias, float eps, void *y,
+                         float *mean, float *rstd, void *stream);
+int zp_layernorm_backward(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx,
+                          int param_dtype, const void *weight, const float *mean, const float *rstd,
+                          const void *dy, int64_t ldy, void *dx, void *dweight, void *dbias, void *work,
+                          size_t work_bytes, void *stream);
+
+/* The join of two layers of a residual network: sum = residual + dropout(x), rounded to the rows' type,
+ * and y = layer norm of sum as it is returned.  p = 0: nothing is dropped, `state` may be NULL.
+ * Backward, from the kept `sum`: dy and dsum are the gradients of the two results (either may be NULL,
+ * not both); dresidual and dx (either may be NULL) those of the two inputs, which for p = 0 are equal. */
+int zp_add_layernorm_forward(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx,
+                             const void *residual, int64_t ldr, double p, const int64_t *state,
+                             int param_dtype, const void *weight, const void *bias, float eps,
+                             void *sum, void *y, float *mean, float *rstd, void *stream);
+int zp_add_layernorm_backward(int64_t rows, int64_t width, int dtype, const void *sum,
+                              int param_dtype, const void *weight, const float *mean,
+                              const float *rstd, const void *dy, int64_t ldy, const void *dsum,
+                              int64_t lds, double p, const int64_t *state, void *dx, void *dresidual,
+                              void *dweight, void *dbias, void *work, size_t work_bytes, void *stream);
+
 /* The energy head after the node output and its VJP (readout, blocks/eso2_ref.py:351-362 and
  * :236-238): rotation invariants of node_out [N, K, C] (the l = 0 row, and per degree l >= 1 the
  * squared norm over m), Linear((lmax+1)C -> C) with weight w0 [C, (lmax+1)C] and bias b0 [C], SiLU,

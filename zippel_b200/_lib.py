@@ -105,6 +105,16 @@ SIGNATURES = {
     "zp_layernorm_silu_forward": (C.c_int, [_I64, C.c_int, _P, _P, _P, C.c_float, _P, _P, _P, _P]),
     "zp_layernorm_silu_backward": (C.c_int, [_I64, C.c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                               _SZ, _P]),
+    "zp_dropout": (C.c_int, [_I64, _I64, C.c_int, _P, _I64, C.c_double, _P, _P, _I64, _P]),
+    "zp_rowwise_work_bytes": (_SZ, [_I64, _I64]),
+    "zp_layernorm_forward": (C.c_int, [_I64, _I64, C.c_int, _P, _I64, C.c_int, _P, _P, C.c_float, _P,
+                                       _P, _P, _P]),
+    "zp_layernorm_backward": (C.c_int, [_I64, _I64, C.c_int, _P, _I64, C.c_int, _P, _P, _P, _P, _I64,
+                                        _P, _P, _P, _P, _SZ, _P]),
+    "zp_add_layernorm_forward": (C.c_int, [_I64, _I64, C.c_int, _P, _I64, _P, _I64, C.c_double, _P,
+                                           C.c_int, _P, _P, C.c_float, _P, _P, _P, _P, _P]),
+    "zp_add_layernorm_backward": (C.c_int, [_I64, _I64, C.c_int, _P, C.c_int, _P, _P, _P, _P, _I64, _P,
+                                            _I64, C.c_double, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "zp_readout_work_bytes": (_SZ, [_P, _I64]),
     "zp_readout_forward": (C.c_int, [_P, _I64] + [_P] * 7 + [_SZ, _P]),
     "zp_readout_backward": (C.c_int, [_P, _I64] + [_P] * 12 + [_SZ, _P]),

@@ -36,6 +36,7 @@ from torch.autograd import forward_ad
 
 from .. import _lib
 from ..graph import EdgeChunk, EdgeGraph
+from . import rowwise
 
 _JD_PATH = __import__("pathlib").Path(__file__).resolve().parent.parent / "data" / "jd.npz"
 
@@ -698,7 +699,9 @@ def tensor_core_linear(plan: Plan, x: torch.Tensor, weight: torch.Tensor, bias) 
 def radial_mlp(plan: Plan, x_edge: torch.Tensor, layers: list) -> torch.Tensor:
     """A ``Linear / LayerNorm / SiLU`` stack (the reference's ``rad_func``) on the library's
     kernels.  ``layers``: modules, or for a functional caller tuples ``("linear", w, b)`` /
-    ``("ln_silu", gamma, beta, eps)``."""
+    ``("ln_silu", gamma, beta, eps)``.  Beyond the reference's stack a ``LayerNorm`` may stand without
+    a ``SiLU`` behind it, ``Dropout`` drops in training, with a state drawn for each call, and
+    ``rowwise.ResidualNorm`` puts a residual around some of the layers."""
     h, i = x_edge, 0
     while i < len(layers):
         m = layers[i]
@@ -712,6 +715,17 @@ def radial_mlp(plan: Plan, x_edge: torch.Tensor, layers: list) -> torch.Tensor:
         elif isinstance(m, nn.LayerNorm) and i + 1 < len(layers) and isinstance(layers[i + 1], nn.SiLU):
             h = LayerNormSiLU.apply(h, m.weight, m.bias, m.eps) if h.shape[0] else h
             i += 2
+        elif isinstance(m, nn.LayerNorm) and len(m.normalized_shape) == 1:
+            params = [None if t is None else t.to(h.dtype) for t in (m.weight, m.bias)]
+            h = rowwise.layer_norm(h, *params, m.eps)
+            i += 1
+        elif isinstance(m, nn.Dropout):
+            if m.training and m.p > 0:
+                h = rowwise.dropout(h, m.p, rowwise.dropout_state(h.device))
+            i += 1
+        elif isinstance(m, rowwise.ResidualNorm):
+            h = m.join(h, radial_mlp(plan, h, list(m.layers)))
+            i += 1
         else:
             raise _lib.ZpError(2, f"radial MLP layer {type(m).__name__} (no kernel for it)")
     return h
