@@ -6,33 +6,12 @@
 //   dropout      y = x / keep where the element is kept, 0 where not (zp_philox.cuh); its VJP is itself
 //   joined       s = residual + dropout(x), rounded to the type;  y = layer norm of s as it is returned
 //     its VJP    gs' = layer norm's VJP of gy + gs;  gresidual = gs';  gx = dropout(gs')
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 #include <cmath>
 
-#include "zp_common.cuh"
-#include "zp_philox.cuh"
-#include "zippel_b200.h"
+#include "zp_rowwise.cuh"
 
 namespace {
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
-
-struct Drop {                       // dropout of a call; state null: nothing is dropped
-  const int64_t *state;
-  uint32_t threshold;
-  float scale;
-};
 
 // sum over a block of kThreads, the same in every thread
 constexpr int kThreads = 256;
@@ -50,7 +29,7 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-dropout_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, Drop drop, T *__restrict__ y,
+dropout_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, ZpDrop drop, T *__restrict__ y,
                int64_t ldy) {
   zp_after_previous();
   const ZpPhiloxKey key = zp_philox_key(drop.state);
@@ -59,21 +38,22 @@ dropout_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx
     const uint32_t kept = zp_philox_kept(key, g, drop.threshold);
     for (int j = 0; j < 8 && 8 * g + j < n; ++j) {
       const int64_t r = (8 * g + j) / width, c = (8 * g + j) % width;
-      y[r * ldy + c] = from_float<T>(kept >> j & 1 ? to_float(x[r * ldx + c]) * drop.scale : 0.f);
+      y[r * ldy + c] = zp_rounded<T>(kept >> j & 1 ? zp_float(x[r * ldx + c]) * drop.scale : 0.f);
     }
   }
 }
 
 template <typename P>
 __device__ __forceinline__ float param(const P *w, int64_t c, float otherwise) {
-  return w ? to_float(w[c]) : otherwise;
+  return w ? zp_float(w[c]) : otherwise;
 }
 
-// one block per row
+// Rows that no team's shared memory holds (above 16384 elements, or where the ring would have one stage):
+// one block per row, passes over global memory.
 template <typename T, typename P>
 __global__ void __launch_bounds__(kThreads)
 norm_fwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, const T *__restrict__ res,
-                int64_t ldr, Drop drop, const P *__restrict__ w, const P *__restrict__ b, float eps,
+                int64_t ldr, ZpDrop drop, const P *__restrict__ w, const P *__restrict__ b, float eps,
                 T *__restrict__ sum, T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
   zp_after_previous();
   __shared__ float red[kThreads / 32];
@@ -84,22 +64,22 @@ norm_fwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ld
       for (int64_t c = threadIdx.x; c < width; c += kThreads) {
         const uint64_t i = (uint64_t)(r * width + c);
         const bool kept = !drop.state || (zp_philox_kept(key, i / 8, drop.threshold) >> (i % 8) & 1);
-        sum[r * width + c] = from_float<T>(to_float(res[r * ldr + c]) +
-                                           (kept ? to_float(in[c]) * drop.scale : 0.f));
+        sum[r * width + c] = zp_rounded<T>(zp_float(res[r * ldr + c]) +
+                                           (kept ? zp_float(in[c]) * drop.scale : 0.f));
       }
       in = sum + r * width;                    // (each thread reads again what it has written)
     }
     float s = 0.f;
-    for (int64_t c = threadIdx.x; c < width; c += kThreads) s += to_float(in[c]);
+    for (int64_t c = threadIdx.x; c < width; c += kThreads) s += zp_float(in[c]);
     const float mean = block_sum(s, red) / (float)width;
     float q = 0.f;
     for (int64_t c = threadIdx.x; c < width; c += kThreads) {
-      const float d = to_float(in[c]) - mean;
+      const float d = zp_float(in[c]) - mean;
       q += d * d;
     }
     const float rstd = rsqrtf(block_sum(q, red) / (float)width + eps);
     for (int64_t c = threadIdx.x; c < width; c += kThreads)
-      y[r * width + c] = from_float<T>((to_float(in[c]) - mean) * rstd * param(w, c, 1.f) + param(b, c, 0.f));
+      y[r * width + c] = zp_rounded<T>((zp_float(in[c]) - mean) * rstd * param(w, c, 1.f) + param(b, c, 0.f));
     if (mean_out && threadIdx.x == 0) { mean_out[r] = mean; rstd_out[r] = rstd; }
   }
 }
@@ -109,7 +89,7 @@ template <typename T, typename P>
 __global__ void __launch_bounds__(kThreads)
 norm_bwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, const P *__restrict__ w,
                 const float *__restrict__ mean_in, const float *__restrict__ rstd_in, const T *__restrict__ dy,
-                int64_t ldy, const T *__restrict__ dsum, int64_t lds, Drop drop, T *__restrict__ dx,
+                int64_t ldy, const T *__restrict__ dsum, int64_t lds, ZpDrop drop, T *__restrict__ dx,
                 T *__restrict__ dres) {
   zp_after_previous();
   __shared__ float red[kThreads / 32];
@@ -117,24 +97,24 @@ norm_bwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ld
     const float mean = mean_in[r], rstd = rstd_in[r];
     float s1 = 0.f, s2 = 0.f;
     for (int64_t c = threadIdx.x; dy && c < width; c += kThreads) {
-      const float gz = to_float(dy[r * ldy + c]) * param(w, c, 1.f);
+      const float gz = zp_float(dy[r * ldy + c]) * param(w, c, 1.f);
       s1 += gz;
-      s2 += gz * ((to_float(x[r * ldx + c]) - mean) * rstd);
+      s2 += gz * ((zp_float(x[r * ldx + c]) - mean) * rstd);
     }
     const float m1 = block_sum(s1, red) / (float)width, m2 = block_sum(s2, red) / (float)width;
     const ZpPhiloxKey key = drop.state ? zp_philox_key(drop.state) : ZpPhiloxKey{};
     for (int64_t c = threadIdx.x; c < width; c += kThreads) {
       float g = 0.f;
       if (dy) {
-        const float z = (to_float(x[r * ldx + c]) - mean) * rstd;
-        g = rstd * (to_float(dy[r * ldy + c]) * param(w, c, 1.f) - m1 - z * m2);
+        const float z = (zp_float(x[r * ldx + c]) - mean) * rstd;
+        g = rstd * (zp_float(dy[r * ldy + c]) * param(w, c, 1.f) - m1 - z * m2);
       }
-      if (dsum) g += to_float(dsum[r * lds + c]);
-      if (dres) dres[r * width + c] = from_float<T>(g);
+      if (dsum) g += zp_float(dsum[r * lds + c]);
+      if (dres) dres[r * width + c] = zp_rounded<T>(g);
       if (dx) {
         const uint64_t i = (uint64_t)(r * width + c);
         const bool kept = !drop.state || (zp_philox_kept(key, i / 8, drop.threshold) >> (i % 8) & 1);
-        dx[r * width + c] = from_float<T>(kept ? g * drop.scale : 0.f);
+        dx[r * width + c] = zp_rounded<T>(kept ? g * drop.scale : 0.f);
       }
     }
   }
@@ -151,36 +131,41 @@ norm_params_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t
   if (c >= width) return;
   float gw = 0.f, gb = 0.f;
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    const float g = to_float(dy[r * ldy + c]);
-    gw += g * ((to_float(x[r * ldx + c]) - mean_in[r]) * rstd_in[r]);
+    const float g = zp_float(dy[r * ldy + c]);
+    gw += g * ((zp_float(x[r * ldx + c]) - mean_in[r]) * rstd_in[r]);
     gb += g;
   }
   partial[(2 * (int64_t)blockIdx.y) * width + c] = gw;
   partial[(2 * (int64_t)blockIdx.y + 1) * width + c] = gb;
 }
 
+// the last sums: 32 columns to a block, the parts dealt out to 32 threads each
 template <typename P>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(1024)
 norm_params_last_kernel(int64_t width, int parts, const float *__restrict__ partial, P *__restrict__ dw,
                         P *__restrict__ db) {
   zp_after_previous();
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= width) return;
-  float gw = 0.f, gb = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    gw += partial[(2 * (int64_t)i) * width + c];
-    gb += partial[(2 * (int64_t)i + 1) * width + c];
-  }
-  if (dw) dw[c] = from_float<P>(gw);
-  if (db) db[c] = from_float<P>(gb);
+  __shared__ float red[32][33];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t c = (int64_t)blockIdx.x * 32 + tx;           // of {gw, gb} side by side
+  float s = 0.f;
+#pragma unroll 4
+  for (int i = ty; i < parts; i += 32) s += c < 2 * width ? partial[(int64_t)i * 2 * width + c] : 0.f;
+  red[ty][tx] = s;
+  __syncthreads();
+  if (ty != 0 || c >= 2 * width) return;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s += red[i][tx];
+  P *const out = c < width ? dw : db;
+  if (out) out[c < width ? c : c - width] = zp_rounded<P>(s);
 }
 
-constexpr int kParts = 148;
 
 bool misplaced(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
 // dropout of probability p (0 <= p <= 1), rounded to a multiple of 2^-16
-bool make_drop(double p, const int64_t *state, Drop &drop) {
+bool make_drop(double p, const int64_t *state, ZpDrop &drop) {
   drop = {nullptr, 0, 1.f};
   if (!(p >= 0.0 && p <= 1.0)) return false;
   drop.threshold = (uint32_t)std::floor(65536.0 * p + 0.5);
@@ -206,7 +191,7 @@ int check_sizes(int64_t rows, int64_t width, int dtype) {
 
 unsigned blocks_for(int64_t n, int64_t most) { return (unsigned)std::max<int64_t>(1, std::min(n, most)); }
 
-template <typename T> int run_dropout(int64_t rows, int64_t width, const void *x, int64_t ldx, const Drop &drop,
+template <typename T> int run_dropout(int64_t rows, int64_t width, const void *x, int64_t ldx, const ZpDrop &drop,
                                       void *y, int64_t ldy, cudaStream_t st) {
   zp_launch(dropout_kernel<T>, blocks_for(zp_ceil_div(rows * width, 8 * kThreads), 148 * 8), kThreads, 0, st, rows,
             width, static_cast<const T *>(x), ldx, drop, static_cast<T *>(y), ldy);
@@ -214,18 +199,10 @@ template <typename T> int run_dropout(int64_t rows, int64_t width, const void *x
   return ZP_OK;
 }
 
-struct NormCall {
-  int64_t rows, width;
-  const void *x, *res, *w, *b, *dy, *dsum;
-  int64_t ldx, ldr, ldy, lds;
-  Drop drop;
-  float eps;
-  const float *mean_in, *rstd_in;
-  void *sum, *y, *dx, *dres, *dw, *db;
-  float *mean, *rstd, *partial;
-};
-
-template <typename T, typename P> int run_fwd(const NormCall &c, cudaStream_t st) {
+template <typename T, typename P> int run_fwd(const ZpNormCall &c, cudaStream_t st) {
+  bool taken = false;
+  if (int rc = zp_launch_norm_fwd(c, taken, st)) return rc;
+  if (taken) return ZP_OK;
   zp_launch(norm_fwd_kernel<T, P>, blocks_for(c.rows, 148 * 8), kThreads, 0, st, c.rows, c.width,
             static_cast<const T *>(c.x), c.ldx, static_cast<const T *>(c.res), c.ldr, c.drop,
             static_cast<const P *>(c.w), static_cast<const P *>(c.b), c.eps, static_cast<T *>(c.sum),
@@ -234,23 +211,27 @@ template <typename T, typename P> int run_fwd(const NormCall &c, cudaStream_t st
   return ZP_OK;
 }
 
-template <typename T, typename P> int run_bwd(const NormCall &c, cudaStream_t st) {
+template <typename T, typename P> int run_bwd(const ZpNormCall &c, cudaStream_t st) {
   const T *x = static_cast<const T *>(c.x), *dy = static_cast<const T *>(c.dy);
-  if (c.dx || c.dres) {
+  bool taken = false;
+  int parts = 0;
+  if (int rc = zp_launch_norm_bwd(c, taken, parts, st)) return rc;
+  if (!taken && (c.dx || c.dres)) {
     zp_launch(norm_bwd_kernel<T, P>, blocks_for(c.rows, 148 * 8), kThreads, 0, st, c.rows, c.width, x, c.ldx,
               static_cast<const P *>(c.w), c.mean_in, c.rstd_in, dy, c.ldy, static_cast<const T *>(c.dsum), c.lds,
               c.drop, static_cast<T *>(c.dx), static_cast<T *>(c.dres));
     ZP_LAUNCH_CHECK("norm_bwd_kernel");
   }
-  if (c.dw || c.db) {
-    const unsigned parts = blocks_for(c.rows, kParts), tiles = (unsigned)zp_ceil_div(c.width, kThreads);
-    zp_launch(norm_params_kernel<T>, dim3(tiles, parts), kThreads, 0, st, c.rows, c.width, x, c.ldx, c.mean_in,
-              c.rstd_in, dy, c.ldy, c.partial);
+  if (!c.partial) return ZP_OK;
+  if (!taken) {
+    parts = (int)blocks_for(c.rows, ZP_ROWWISE_PARTS);
+    zp_launch(norm_params_kernel<T>, dim3((unsigned)zp_ceil_div(c.width, kThreads), parts), kThreads, 0, st, c.rows,
+              c.width, x, c.ldx, c.mean_in, c.rstd_in, dy, c.ldy, c.partial);
     ZP_LAUNCH_CHECK("norm_params_kernel");
-    zp_launch(norm_params_last_kernel<P>, tiles, kThreads, 0, st, c.width, (int)parts, c.partial,
-              static_cast<P *>(c.dw), static_cast<P *>(c.db));
-    ZP_LAUNCH_CHECK("norm_params_last_kernel");
   }
+  zp_launch(norm_params_last_kernel<P>, (unsigned)zp_ceil_div(2 * c.width, 32), 1024, 0, st, c.width, parts, c.partial,
+            static_cast<P *>(c.dw), static_cast<P *>(c.db));
+  ZP_LAUNCH_CHECK("norm_params_last_kernel");
   return ZP_OK;
 }
 
@@ -264,13 +245,13 @@ template <typename T, typename P> int run_bwd(const NormCall &c, cudaStream_t st
                                    : CALL<__nv_bfloat16, __nv_bfloat16>(c, st);     \
   }
 
-int norm_fwd(const NormCall &c, int dtype, int param_dtype, cudaStream_t st) { BY_TYPES(run_fwd) }
-int norm_bwd(const NormCall &c, int dtype, int param_dtype, cudaStream_t st) { BY_TYPES(run_bwd) }
+int norm_fwd(ZpNormCall &c, int dtype, int param_dtype, cudaStream_t st) { c.dtype = dtype; c.param_dtype = param_dtype; BY_TYPES(run_fwd) }
+int norm_bwd(ZpNormCall &c, int dtype, int param_dtype, void *work, cudaStream_t st) { c.dtype = dtype; c.param_dtype = param_dtype; c.partial = c.dw || c.db ? static_cast<float *>(work) : nullptr; BY_TYPES(run_bwd) }
 #undef BY_TYPES
 
 bool bad_param_type(int dtype, int param_dtype) { return param_dtype != dtype && param_dtype != ZP_F32; }
 
-int check_fwd(const NormCall &c, int dtype, int param_dtype) {
+int check_fwd(const ZpNormCall &c, int dtype, int param_dtype) {
   if (bad_param_type(dtype, param_dtype)) return ZP_ERR_UNSUPPORTED;
   if (bad_rows(c.x, c.rows, c.width, c.ldx, dtype) || bad_rows(c.y, c.rows, c.width, c.width, dtype) ||
       misplaced(c.w, type_bytes(param_dtype)) || misplaced(c.b, type_bytes(param_dtype)) ||
@@ -279,14 +260,14 @@ int check_fwd(const NormCall &c, int dtype, int param_dtype) {
   return ZP_OK;
 }
 
-int zero_params(const NormCall &c, int param_dtype, cudaStream_t st) {
+int zero_params(const ZpNormCall &c, int param_dtype, cudaStream_t st) {
   const size_t bytes = (size_t)c.width * type_bytes(param_dtype);
   if (c.dw) ZP_CUDA(cudaMemsetAsync(c.dw, 0, bytes, st));
   if (c.db) ZP_CUDA(cudaMemsetAsync(c.db, 0, bytes, st));
   return ZP_OK;
 }
 
-int check_bwd(const NormCall &c, int dtype, int param_dtype, const void *work, size_t work_bytes) {
+int check_bwd(const ZpNormCall &c, int dtype, int param_dtype, const void *work, size_t work_bytes) {
   const size_t size = type_bytes(dtype), psize = type_bytes(param_dtype);
   if (bad_rows(c.x, c.rows, c.width, c.ldx, dtype) || (c.dy && bad_rows(c.dy, c.rows, c.width, c.ldy, dtype)) ||
       !c.mean_in || !c.rstd_in || misplaced(c.mean_in, 4) || misplaced(c.rstd_in, 4) || misplaced(c.w, psize) ||
@@ -306,7 +287,7 @@ extern "C" {
 int zp_dropout(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx, double p, const int64_t *state,
                void *y, int64_t ldy, void *stream) {
   if (int rc = check_sizes(rows, width, dtype)) return rc;
-  Drop drop;
+  ZpDrop drop;
   if (rows == 0) return p >= 0.0 && p <= 1.0 ? ZP_OK : ZP_ERR_INVALID_ARG;
   if (!make_drop(p, state, drop) || !state || misplaced(state, 8) || bad_rows(x, rows, width, ldx, dtype) ||
       bad_rows(y, rows, width, ldy, dtype))
@@ -319,7 +300,7 @@ int zp_dropout(int64_t rows, int64_t width, int dtype, const void *x, int64_t ld
 }
 
 size_t zp_rowwise_work_bytes(int64_t rows, int64_t width) {
-  return rows > 0 && width > 0 ? sizeof(float) * 2 * (size_t)std::min<int64_t>(rows, kParts) * (size_t)width : 0;
+  return rows > 0 && width > 0 ? sizeof(float) * 2 * (size_t)std::min<int64_t>(rows, ZP_ROWWISE_PARTS) * (size_t)width : 0;
 }
 
 int zp_layernorm_forward(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx, int param_dtype,
@@ -327,7 +308,7 @@ int zp_layernorm_forward(int64_t rows, int64_t width, int dtype, const void *x, 
                          void *stream) {
   if (int rc = check_sizes(rows, width, dtype)) return rc;
   if (rows == 0) return ZP_OK;
-  NormCall c = {};
+  ZpNormCall c = {};
   c.rows = rows; c.width = width; c.x = x; c.ldx = ldx; c.w = weight; c.b = bias; c.eps = eps; c.y = y;
   c.mean = mean; c.rstd = rstd; c.drop.scale = 1.f;
   if (int rc = check_fwd(c, dtype, param_dtype)) return rc;
@@ -339,15 +320,15 @@ int zp_layernorm_backward(int64_t rows, int64_t width, int dtype, const void *x,
                           void *dx, void *dweight, void *dbias, void *work, size_t work_bytes, void *stream) {
   if (int rc = check_sizes(rows, width, dtype)) return rc;
   if (bad_param_type(dtype, param_dtype)) return ZP_ERR_UNSUPPORTED;
-  NormCall c = {};
+  ZpNormCall c = {};
   c.rows = rows; c.width = width; c.x = x; c.ldx = ldx; c.w = weight; c.mean_in = mean; c.rstd_in = rstd;
-  c.dy = dy; c.ldy = ldy; c.dx = dx; c.dw = dweight; c.db = dbias; c.partial = static_cast<float *>(work);
+  c.dy = dy; c.ldy = ldy; c.dx = dx; c.dw = dweight; c.db = dbias;
   c.drop.scale = 1.f;
   cudaStream_t st = (cudaStream_t)stream;
   if (rows == 0) return zero_params(c, param_dtype, st);
   if (!dy) return ZP_ERR_INVALID_ARG;
   if (int rc = check_bwd(c, dtype, param_dtype, work, work_bytes)) return rc;
-  return norm_bwd(c, dtype, param_dtype, st);
+  return norm_bwd(c, dtype, param_dtype, work, st);
 }
 
 int zp_add_layernorm_forward(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx,
@@ -355,7 +336,7 @@ int zp_add_layernorm_forward(int64_t rows, int64_t width, int dtype, const void 
                              const void *weight, const void *bias, float eps, void *sum, void *y, float *mean,
                              float *rstd, void *stream) {
   if (int rc = check_sizes(rows, width, dtype)) return rc;
-  NormCall c = {};
+  ZpNormCall c = {};
   if (rows == 0) return p >= 0.0 && p <= 1.0 ? ZP_OK : ZP_ERR_INVALID_ARG;
   if (!make_drop(p, state, c.drop)) return ZP_ERR_INVALID_ARG;
   c.rows = rows; c.width = width; c.x = x; c.ldx = ldx; c.res = residual; c.ldr = ldr; c.w = weight; c.b = bias;
@@ -373,10 +354,10 @@ int zp_add_layernorm_backward(int64_t rows, int64_t width, int dtype, const void
                               void *stream) {
   if (int rc = check_sizes(rows, width, dtype)) return rc;
   if (bad_param_type(dtype, param_dtype)) return ZP_ERR_UNSUPPORTED;
-  NormCall c = {};
+  ZpNormCall c = {};
   c.rows = rows; c.width = width; c.x = sum; c.ldx = width; c.w = weight; c.mean_in = mean; c.rstd_in = rstd;
   c.dy = dy; c.ldy = ldy; c.dsum = dsum; c.lds = lds; c.dx = dx; c.dres = dresidual; c.dw = dweight; c.db = dbias;
-  c.partial = static_cast<float *>(work);
+ 
   cudaStream_t st = (cudaStream_t)stream;
   if (rows == 0) return p >= 0.0 && p <= 1.0 ? zero_params(c, param_dtype, st) : (int)ZP_ERR_INVALID_ARG;
   if (!make_drop(p, state, c.drop)) return ZP_ERR_INVALID_ARG;
@@ -388,7 +369,7 @@ int zp_add_layernorm_backward(int64_t rows, int64_t width, int dtype, const void
     c.dw = c.db = nullptr;
     if (!dx && !dresidual) return ZP_OK;
   }
-  return norm_bwd(c, dtype, param_dtype, st);
+  return norm_bwd(c, dtype, param_dtype, work, st);
 }
 
 }  // extern "C"
