@@ -13,6 +13,8 @@
 
 namespace {
 
+bool misplaced(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
 // sum over a block of kThreads, the same in every thread
 constexpr int kThreads = 256;
 __device__ __forceinline__ float block_sum(float v, float *red) {
@@ -27,18 +29,97 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
   return s;
 }
 
+// Dropout where groups of eight elements (one counter's) lie in aligned pieces of 16 bytes: `per_row`
+// groups a row, a warp 32 kAhead pieces at a time.  Bound by memory, with the generator close behind: of
+// some 75 integer instructions per group 20 are wide products.  In fp32 a piece is half a group: of two
+// neighbouring lanes each works out the counter of one of two pieces, and they swap.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-dropout_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, ZpDrop drop, T *__restrict__ y,
-               int64_t ldy) {
+dropout_pieces_kernel(int64_t groups, uint32_t per_row, const T *__restrict__ x, int64_t ldx, ZpDrop drop,
+                      T *__restrict__ y, int64_t ldy) {
+  zp_after_previous();
+  constexpr int kAhead = 4, V = kZpVec<T>, kPieces = 8 / V;        // pieces of a group
+  const ZpPhiloxKey key = zp_philox_key(drop.state);
+  const int lane = threadIdx.x % 32;
+  const int64_t pieces = groups * kPieces, step = (int64_t)gridDim.x * kThreads * kAhead;
+  const bool flat = per_row == 0, small = groups <= 0xffffffffll;
+  for (int64_t p0 = (int64_t)(blockIdx.x * kThreads + threadIdx.x - lane) * kAhead; p0 < pieces; p0 += step) {
+    uint4 in[kAhead];
+    int64_t to[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t p = p0 + 32 * i + lane;
+      if (p >= pieces) continue;
+      int64_t from = p * V;
+      to[i] = p * V;
+      if (!flat) {
+        const int64_t g = p / kPieces, r = small ? (uint32_t)g / per_row : g / per_row;
+        const int64_t c = (g - r * per_row) * 8 + p % kPieces * V;
+        from = r * ldx + c;
+        to[i] = r * ldy + c;
+      }
+      in[i] = __ldcs(reinterpret_cast<const uint4 *>(x + from));
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; i += kPieces) {
+      uint32_t kept[kPieces];
+      if constexpr (kPieces == 1) {
+        kept[0] = zp_philox_kept(key, p0 + 32 * i + lane, drop.threshold);
+      } else {
+        const int odd = lane & 1;
+        const uint32_t mine = zp_philox_kept(key, (p0 + 32 * (i + odd) + lane) / 2, drop.threshold);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+        kept[0] = odd ? other >> 4 : mine;
+        kept[1] = odd ? mine >> 4 : other;
+      }
+#pragma unroll
+      for (int h = 0; h < kPieces; ++h) {
+        if (p0 + 32 * (i + h) + lane >= pieces) continue;
+        float v[V];
+        zp_unpack<T>(in[i + h], v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = kept[h] >> k & 1 ? v[k] * drop.scale : 0.f;
+        __stcs(reinterpret_cast<uint4 *>(y + to[i + h]), zp_pack<T>(v));
+      }
+    }
+  }
+}
+
+// Elements first .. rows * width - 1 wherever they lie: a warp goes through 256 of them, works out the 32
+// counters and hands each lane its bits; element by element the accesses are still side by side.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+dropout_elements_kernel(int64_t first, int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, ZpDrop drop,
+                        T *__restrict__ y, int64_t ldy) {
   zp_after_previous();
   const ZpPhiloxKey key = zp_philox_key(drop.state);
-  const int64_t n = rows * width, groups = (n + 7) / 8;
-  for (int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x; g < groups; g += (int64_t)gridDim.x * kThreads) {
-    const uint32_t kept = zp_philox_kept(key, g, drop.threshold);
-    for (int j = 0; j < 8 && 8 * g + j < n; ++j) {
-      const int64_t r = (8 * g + j) / width, c = (8 * g + j) % width;
-      y[r * ldy + c] = zp_rounded<T>(kept >> j & 1 ? zp_float(x[r * ldx + c]) * drop.scale : 0.f);
+  const int lane = threadIdx.x % 32;
+  const int64_t n = rows * width, step = (int64_t)gridDim.x * kThreads * 8;
+  for (int64_t e0 = first + (int64_t)(blockIdx.x * kThreads + threadIdx.x - lane) * 8; e0 < n; e0 += step) {
+    float v[8];
+    int64_t to[8];
+    int64_t r = 0, c = e0 + lane;
+    if (rows > 1) {
+      r = n <= 0xffffffffll ? (uint32_t)c / (uint32_t)width : c / width;
+      c -= r * width;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = 0.f;
+      to[j] = r * ldy + c;
+      if (e0 + 32 * j + lane < n) v[j] = zp_float(x[r * ldx + c]);
+      c += 32;
+      if (c >= width && rows > 1) {
+        const int64_t more = width > 32 ? 1 : c / width;
+        r += more;
+        c -= more * width;
+      }
+    }
+    const uint32_t mine = zp_philox_kept(key, e0 / 8 + lane, drop.threshold);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t kept = __shfl_sync(0xffffffffu, mine, 4 * j + lane / 8) >> (lane % 8) & 1;
+      if (e0 + 32 * j + lane < n) y[to[j]] = zp_rounded<T>(kept ? v[j] * drop.scale : 0.f);
     }
   }
 }
@@ -162,8 +243,6 @@ norm_params_last_kernel(int64_t width, int parts, const float *__restrict__ part
 }
 
 
-bool misplaced(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
-
 // dropout of probability p (0 <= p <= 1), rounded to a multiple of 2^-16
 bool make_drop(double p, const int64_t *state, ZpDrop &drop) {
   drop = {nullptr, 0, 1.f};
@@ -193,9 +272,31 @@ unsigned blocks_for(int64_t n, int64_t most) { return (unsigned)std::max<int64_t
 
 template <typename T> int run_dropout(int64_t rows, int64_t width, const void *x, int64_t ldx, const ZpDrop &drop,
                                       void *y, int64_t ldy, cudaStream_t st) {
-  zp_launch(dropout_kernel<T>, blocks_for(zp_ceil_div(rows * width, 8 * kThreads), 148 * 8), kThreads, 0, st, rows,
-            width, static_cast<const T *>(x), ldx, drop, static_cast<T *>(y), ldy);
-  ZP_LAUNCH_CHECK("dropout_kernel");
+  const T *in = static_cast<const T *>(x);
+  T *out = static_cast<T *>(y);
+  if ((ldx == width && ldy == width) || rows == 1) {         // one row, and all of it that is whole groups
+    width *= rows;
+    rows = 1;
+    ldx = ldy = width;
+  }
+  const bool pieces = !misplaced(x, 16) && !misplaced(y, 16) &&
+                      (rows == 1 || (width % 8 == 0 && width / 8 <= 0xffffffffll && ldx * sizeof(T) % 16 == 0 &&
+                                     ldy * sizeof(T) % 16 == 0));
+  int64_t first = 0;
+  if (pieces) {
+    const int64_t groups = rows * width / 8;
+    first = groups * 8;
+    if (groups > 0) {
+      zp_launch(dropout_pieces_kernel<T>, blocks_for(zp_ceil_div(groups * (8 / kZpVec<T>), 4 * kThreads), 148 * 8),
+                kThreads, 0, st, groups, rows == 1 ? 0u : (uint32_t)(width / 8), in, ldx, drop, out, ldy);
+      ZP_LAUNCH_CHECK("dropout_pieces_kernel");
+    }
+  }
+  if (first < rows * width) {
+    zp_launch(dropout_elements_kernel<T>, blocks_for(zp_ceil_div(rows * width - first, 8 * kThreads), 148 * 8), kThreads,
+              0, st, first, rows, width, in, ldx, drop, out, ldy);
+    ZP_LAUNCH_CHECK("dropout_elements_kernel");
+  }
   return ZP_OK;
 }
 

@@ -39,7 +39,7 @@ struct ZpNormCall {
 // The kernels of teams (zp_rowwise_fwd.cu, zp_rowwise_bwd.cu); `taken` false: the call is not for them
 // and nothing was launched.  The backward leaves `parts` rows of partial sums {gw, gb} in c.partial, at
 // most ZP_ROWWISE_PARTS.
-#define ZP_ROWWISE_PARTS 296
+#define ZP_ROWWISE_PARTS 148
 int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st);
 int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_t st);
 
@@ -126,8 +126,9 @@ struct ZpTeam {
   // sums over the team, the same in all of it; `turn` alternates from sum to sum (a buffer that is
   // written again has been read by all: the other's barrier lies in between)
   __device__ __forceinline__ float2 sum(float2 v, int turn) const {
-    const int steps = size < 32 ? size : 32;
-    for (int o = steps >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      if (o >= size) continue;
       v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
       v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
@@ -135,26 +136,30 @@ struct ZpTeam {
     float2 *at = red + (turn & 1) * (kZpTeamThreads / 32);
     if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
     sync();
-    const int first = index * (size >> 5), n = size >> 5;
-    float2 s = make_float2(0.f, 0.f);
-    for (int w = 0; w < n; ++w) {
-      const float2 p = at[first + w];
-      s.x += p.x;
-      s.y += p.y;
+    const int n = size >> 5;                   // warps: each adds up all of them, in the same order
+    v = at[index * n + (threadIdx.x & (n - 1))];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      if (o >= n) continue;
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
-    return s;
+    return v;
   }
   __device__ __forceinline__ float sum(float v, int turn) const {
-    const int steps = size < 32 ? size : 32;
-    for (int o = steps >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (o < size) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (size <= 32) return v;
     float *at = reinterpret_cast<float *>(red + (turn & 1) * (kZpTeamThreads / 32));
     if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
     sync();
-    const int first = index * (size >> 5), n = size >> 5;
-    float s = 0.f;
-    for (int w = 0; w < n; ++w) s += at[first + w];
-    return s;
+    const int n = size >> 5;
+    v = at[index * n + (threadIdx.x & (n - 1))];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+      if (o < n) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
   }
 };
 
@@ -164,45 +169,50 @@ __device__ __forceinline__ void zp_copy16(uint32_t to, const void *from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void zp_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// until at most `pending` of this thread's latest groups are on their way
-__device__ __forceinline__ void zp_copy_wait(int pending) {
-  switch (pending) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-  }
+// until of this thread's latest groups at most `stages` - 2 are on their way (stages: 2 or 4)
+__device__ __forceinline__ void zp_copy_wait(int stages) {
+  if (stages == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
-constexpr int kZpMostStages = 8;
 
-// One of the arrays that a ring brings in.  first / last: the addresses that may be read.
+// One of the arrays that a ring brings in: the next row to fetch, and the addresses that may be read.
 struct ZpSource {
-  const char *base;
-  int64_t ld;                                  // bytes between two rows
-  const char *last;                            // one past the last row's last byte
+  const char *row, *begin, *end;
+  int64_t step;                                // bytes from a team's row to its next
+  int place, turn;                             // of the row that is worked on within 16 bytes; added per row
+  __device__ __forceinline__ ZpSource(const void *base, int64_t ld, int64_t rows, int64_t width, int size,
+                                      int64_t first, int64_t rows_per_step) {
+    begin = static_cast<const char *>(base);
+    end = begin + ((rows - 1) * ld + width) * size;
+    row = begin + first * ld * size;
+    step = rows_per_step * ld * size;
+    place = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+    turn = (int)(step & 15);
+  }
+  __device__ __forceinline__ void advance() { place = (place + turn) & 15; }
 };
 
-// Row of `width` elements of T into a slot.  kAligned: element c goes to byte c * sizeof(T), each thread
-// copies its own.  Else the row keeps its place within 16 bytes; returns that place.
+// The next row of `width` elements of T into a slot.  kAligned: element c goes to byte c * sizeof(T), each
+// thread copies its own.  Else the row keeps its place within 16 bytes.
 template <typename T, bool kAligned, int E>
-__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, char *slot, const ZpSource &s, int64_t r, int width) {
-  const char *row = s.base + r * s.ld;
+__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, char *slot, ZpSource &s, bool live, int width) {
+  const char *const row = s.row;
+  s.row += s.step;
+  if (!live) return;
   if constexpr (kAligned) {
-    const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot);
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot) + 16 * t.lane;
+    const char *const from = row + 16 * t.lane;
 #pragma unroll
     for (int i = 0; i < E / kZpVec<T>; ++i) {
       const int piece = t.lane + i * t.size;
-      if (piece * kZpVec<T> < width) zp_copy16(to + 16 * piece, row + 16 * (int64_t)piece);
+      if (piece * kZpVec<T> < width) zp_copy16(to + 16 * i * t.size, from + 16 * i * t.size);
     }
   } else {
     const char *from = reinterpret_cast<const char *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
-    const char *end = row + (int64_t)width * sizeof(T);
+    const char *end = row + width * (int)sizeof(T);
     for (const char *p = from + 16 * t.lane; p < end; p += 16 * t.size) {
       char *to = slot + (p - from);
-      if (p >= s.base && p + 16 <= s.last) {
+      if (p >= s.begin && p + 16 <= s.end) {
         zp_copy16((uint32_t)__cvta_generic_to_shared(to), p);
       } else {                                 // the ends of the array: what lies outside is not read
         for (int k = 0; k < 16; k += sizeof(T))
@@ -211,9 +221,6 @@ __device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, char *slot, const 
       }
     }
   }
-}
-template <typename T, bool kAligned> __device__ __forceinline__ int zp_row_place(const ZpSource &s, int64_t r) {
-  return kAligned ? 0 : (int)(reinterpret_cast<uintptr_t>(s.base + r * s.ld) & 15);
 }
 
 // A thread's V elements number i of a row in a slot (kAligned: a piece of 16 bytes, else one element)
@@ -285,31 +292,32 @@ struct ZpTeamPlan {
   size_t smem;
   unsigned blocks;
 };
-// `arrays` come in per row; `floor_bytes`: shared memory that the kernel needs besides, after the ring is
-// done with; false: the rows are too wide
-inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, size_t floor_bytes_per_element,
+// `arrays` come in per row; `last_per_element`: bytes of shared memory per element of a block's teams that
+// the kernel needs when the ring is done with; `most`: elements of a thread where there are rows enough.
+// False: the rows are too wide.
+inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, size_t last_per_element, int most,
                          ZpTeamPlan &p) {
-  const size_t size = c.dtype == ZP_F32 ? 4 : 2;
+  const int64_t size = c.dtype == ZP_F32 ? 4 : 2;
   if (c.width > kZpTeamThreads * 32) return false;
   p.aligned = aligned;
-  const int64_t need = zp_ceil_div(c.width, 8);
-  for (p.team = 2; p.team < need && p.team < kZpTeamThreads; p.team *= 2) {}
-  for (p.elements = 8; (int64_t)p.team * p.elements < c.width; p.elements *= 2) {}
+  for (p.elements = 8; p.elements < 32; p.elements *= 2) {
+    if (c.width > (int64_t)kZpTeamThreads * p.elements) continue;
+    if (p.elements >= most || c.rows * c.width < (int64_t)148 * kZpTeamThreads * 2 * p.elements) break;
+  }
+  const int64_t need = zp_ceil_div(c.width, p.elements);
+  for (p.team = 2; p.team < need; p.team *= 2) {}
   const int teams = kZpTeamThreads / p.team;
-  p.slot = (int)zp_align_up((size_t)p.team * p.elements * size + (aligned ? 0 : 16), 16);
+  p.slot = (int)zp_align_up((size_t)(p.team * p.elements * size) + (aligned ? 0 : 16), 16);
   p.bytes = aligned || !c.drop.state ? 0 : (int)zp_align_up((size_t)c.width / 8 + 2, 16);
   const size_t red = 2 * sizeof(float2) * (kZpTeamThreads / 32), fixed = red + (size_t)p.bytes * teams;
-  const size_t last = floor_bytes_per_element * kZpTeamThreads * p.elements;
+  const size_t last = last_per_element * kZpTeamThreads * p.elements;
   const size_t stage = (size_t)arrays * p.slot * teams;
-  const int resident = p.elements == 8 ? 2 : 1;
-  const size_t room = (size_t)(226 * 1024) / resident - 1024;
-  p.stages = 0;
-  for (int d = 2; d <= kZpMostStages && fixed + d * stage <= room && (d <= 4 || d * stage <= 48 * 1024); ++d)
-    p.stages = d;
-  if (!p.stages || fixed + last > room) return false;
+  const size_t room = 226 * 1024;
+  p.stages = fixed + 4 * stage <= room ? 4 : 2;
+  if (fixed + p.stages * stage > room || fixed + last > room) return false;
   p.smem = fixed + (p.stages * stage > last ? p.stages * stage : last);
   const int64_t units = zp_ceil_div(c.rows, p.team < 32 ? 32 / p.team : 1);
-  p.blocks = (unsigned)(units < 148 * resident ? units : 148 * resident);
+  p.blocks = (unsigned)(units < 148 ? units : 148);
   return true;
 }
 inline bool zp_piece_aligned(const void *p, int64_t ld, size_t size) {

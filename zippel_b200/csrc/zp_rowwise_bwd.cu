@@ -9,11 +9,11 @@
 namespace {
 
 template <typename T, bool kAligned, int E, bool kJoin>
-__global__ void __launch_bounds__(kZpTeamThreads, E == 8 ? 2 : 1)
+__global__ void __launch_bounds__(kZpTeamThreads, 1)
 norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
   zp_after_previous();
   constexpr int V = kZpStep<T, kAligned>, M = E / V;
-  constexpr bool kHeld = E <= 16;
+  constexpr bool kHeld = E <= 16, kKept = E <= 16;
   extern __shared__ __align__(16) char smem[];
   const ZpTeam t(p.team, reinterpret_cast<float2 *>(smem));
   const int width = (int)c.width, teams = kZpTeamThreads / p.team, stages = p.stages;
@@ -22,24 +22,22 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
   char *const rings = after_red + p.bytes * teams;
   const int A = kJoin && c.dsum ? 3 : 2;
   char *const ring = rings + (size_t)t.index * stages * A * p.slot;
-  const int64_t size = sizeof(T);
-  auto source = [&](const void *base, int64_t ld) {
-    const char *at = static_cast<const char *>(base);
-    return ZpSource{at, ld * size, at + ((c.rows - 1) * ld + c.width) * size};
-  };
-  const ZpSource sx = source(c.x, c.ldx), sy = source(c.dy, c.ldy), ss = source(c.dsum, c.lds);
   const int64_t step = (int64_t)gridDim.x * t.walkers * t.per;
   const int64_t first = ((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per + t.sub;
-  auto fetch = [&](int64_t r, int stage) {
-    if (r < c.rows) {
-      char *to = ring + stage * A * p.slot;
-      zp_fetch_row<T, kAligned, E>(t, to, sx, r, width);
-      zp_fetch_row<T, kAligned, E>(t, to + p.slot, sy, r, width);
-      if (kJoin && A == 3) zp_fetch_row<T, kAligned, E>(t, to + 2 * p.slot, ss, r, width);
-    }
+  ZpSource sx(c.x, c.ldx, c.rows, c.width, sizeof(T), first, step);
+  ZpSource sy(c.dy, c.ldy, c.rows, c.width, sizeof(T), first, step);
+  ZpSource ss(c.dsum, c.lds, c.rows, c.width, sizeof(T), first, step);
+  int64_t coming = first;
+  auto fetch = [&](int stage) {
+    char *const to = ring + stage * A * p.slot;
+    const bool live = coming < c.rows;
+    zp_fetch_row<T, kAligned, E>(t, to, sx, live, width);
+    zp_fetch_row<T, kAligned, E>(t, to + p.slot, sy, live, width);
+    if (kJoin && A == 3) zp_fetch_row<T, kAligned, E>(t, to + 2 * p.slot, ss, live, width);
+    coming += step;
     zp_copy_commit();
   };
-  for (int s = 0; s < stages - 1; ++s) fetch(first + s * step, s);
+  for (int s = 0; s < stages - 1; ++s) fetch(s);
 
   const bool wide = c.param_dtype == ZP_F32;
   auto column = [&](int i, int k) { return (t.lane + i * t.size) * V + k; };
@@ -59,17 +57,21 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
     const int64_t r = base + t.sub;
     const bool live = r < c.rows;
     const float mean = next_mean, rstd = next_rstd;
-    zp_copy_wait(stages - 2);
+    zp_copy_wait(stages);
     if (!kAligned) t.sync();
-    fetch(r + (stages - 1) * step, stage == 0 ? stages - 1 : stage - 1);
+    fetch(stage == 0 ? stages - 1 : stage - 1);
     if (r + step < c.rows) { next_mean = c.mean_in[r + step]; next_rstd = c.rstd_in[r + step]; }
     const char *const slot = ring + stage * A * p.slot;
-    const char *const x = slot + zp_row_place<T, kAligned>(sx, r);
-    const char *const dy = slot + p.slot + zp_row_place<T, kAligned>(sy, r);
-    const char *const ds = slot + 2 * p.slot + zp_row_place<T, kAligned>(ss, r);
+    const char *const x = slot + (kAligned ? 0 : sx.place);
+    const char *const dy = slot + p.slot + (kAligned ? 0 : sy.place);
+    const char *const ds = slot + 2 * p.slot + (kAligned ? 0 : ss.place);
+    sx.advance();
+    sy.advance();
+    ss.advance();
     stage = stage + 1 == stages ? 0 : stage + 1;
     const int mine = live ? width : 0;
     float2 s = make_float2(0.f, 0.f);
+    float zs[kKept ? E : 1], gs[kKept ? E : 1];          // z and gy w, where there are registers for them
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       if (column(i, 0) >= mine) continue;
@@ -83,6 +85,7 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
         gb[i * V + k] += g[k];
         s.x += gz;
         s.y += gz * z;
+        if constexpr (kKept) { zs[i * V + k] = z; gs[i * V + k] = gz; }
       }
     }
     s = t.sum(s, turn++);
@@ -94,12 +97,14 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
     for (int i = 0; i < M; ++i) {
       if (column(i, 0) >= mine) continue;
       float v[V], g[V];
-      zp_read<T, kAligned>(t, x, i, v);
-      zp_read<T, kAligned>(t, dy, i, g);
+      if constexpr (kKept) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float z = (v[k] - mean) * rstd;
-        v[k] = rstd * (g[k] * weight(i, k) - m1 - z * m2);
+        for (int k = 0; k < V; ++k) v[k] = rstd * (gs[i * V + k] - m1 - zs[i * V + k] * m2);
+      } else {
+        zp_read<T, kAligned>(t, x, i, v);
+        zp_read<T, kAligned>(t, dy, i, g);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = rstd * (g[k] * weight(i, k) - m1 - (v[k] - mean) * rstd * m2);
       }
       if constexpr (kJoin) {
         if (A == 3) {
@@ -117,7 +122,7 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
       }
     }
   }
-  zp_copy_wait(0);
+  zp_copy_wait(2);
   if (!c.partial) return;
   // teams within a warp first, then those of the block (`copies` of them) through shared memory, in order
   for (int o = t.size; o < 32; o <<= 1) {
@@ -181,7 +186,7 @@ int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_
                        (!c.dres || zp_piece_aligned(c.dres, c.width, size)) &&
                        (!c.drop.state || c.width % 8 == 0);
   ZpTeamPlan p;
-  taken = c.dy && zp_team_plan(c, aligned, c.dsum ? 3 : 2, c.partial ? 2 * sizeof(float) : 0, p);
+  taken = c.dy && zp_team_plan(c, aligned, c.dsum ? 3 : 2, c.partial ? 2 * sizeof(float) : 0, 16, p);
   if (!taken) return ZP_OK;
   parts = (int)p.blocks;
   if (c.dtype == ZP_F32) return by_alignment<float>(c, p, st);

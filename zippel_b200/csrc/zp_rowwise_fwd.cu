@@ -9,45 +9,39 @@
 namespace {
 
 template <typename T, bool kAligned, int E, bool kJoin>
-__global__ void __launch_bounds__(kZpTeamThreads, E == 8 ? 2 : 1)
+__global__ void __launch_bounds__(kZpTeamThreads, 1)
 norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
   zp_after_previous();
   constexpr int V = kZpStep<T, kAligned>, M = E / V, A = kJoin ? 2 : 1;
-  constexpr bool kHeld = E <= 16;              // weight and bias stay in registers
   extern __shared__ __align__(16) char smem[];
   const ZpTeam t(p.team, reinterpret_cast<float2 *>(smem));
   const int width = (int)c.width, teams = kZpTeamThreads / p.team, stages = p.stages;
   char *const after_red = smem + 2 * sizeof(float2) * (kZpTeamThreads / 32);
   uint8_t *const bytes = reinterpret_cast<uint8_t *>(after_red) + t.index * p.bytes;
   char *const ring = after_red + p.bytes * teams + (size_t)t.index * stages * A * p.slot;
-  const int64_t size = sizeof(T);
-  const ZpSource src[2] = {
-      {static_cast<const char *>(c.x), c.ldx * size,
-       static_cast<const char *>(c.x) + ((c.rows - 1) * c.ldx + c.width) * size},
-      {static_cast<const char *>(c.res), c.ldr * size,
-       static_cast<const char *>(c.res) + ((c.rows - 1) * c.ldr + c.width) * size}};
   const int64_t step = (int64_t)gridDim.x * t.walkers * t.per;
   const int64_t first = ((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per + t.sub;
-  auto fetch = [&](int64_t r, int stage) {
-    if (r < c.rows) {
-#pragma unroll
-      for (int a = 0; a < A; ++a)
-        zp_fetch_row<T, kAligned, E>(t, ring + (stage * A + a) * p.slot, src[a], r, width);
-    }
+  ZpSource sx(c.x, c.ldx, c.rows, c.width, sizeof(T), first, step);
+  ZpSource sr(c.res, c.ldr, c.rows, c.width, sizeof(T), first, step);
+  int64_t coming = first;
+  auto fetch = [&](int stage) {
+    char *const to = ring + stage * A * p.slot;
+    zp_fetch_row<T, kAligned, E>(t, to, sx, coming < c.rows, width);
+    if (kJoin) zp_fetch_row<T, kAligned, E>(t, to + p.slot, sr, coming < c.rows, width);
+    coming += step;
     zp_copy_commit();
   };
-  for (int s = 0; s < stages - 1; ++s) fetch(first + s * step, s);
+  for (int s = 0; s < stages - 1; ++s) fetch(s);
 
   const bool wide = c.param_dtype == ZP_F32;
-  float w[kHeld ? E : 1], b[kHeld ? E : 1];
   auto column = [&](int i, int k) { return (t.lane + i * t.size) * V + k; };
-  if constexpr (kHeld) {
+  constexpr bool kHeld = E <= 16;              // weight and bias stay in registers
+  float w[kHeld ? E : 1], b[kHeld ? E : 1];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int col = column(e / V, e % V);
-      w[e] = col < width ? zp_param<T>(c.w, wide, col, 1.f) : 0.f;
-      b[e] = col < width ? zp_param<T>(c.b, wide, col, 0.f) : 0.f;
-    }
+  for (int e = 0; e < (kHeld ? E : 0); ++e) {
+    const int col = column(e / V, e % V);
+    w[e] = col < width ? zp_param<T>(c.w, wide, col, 1.f) : 0.f;
+    b[e] = col < width ? zp_param<T>(c.b, wide, col, 0.f) : 0.f;
   }
   const ZpPhiloxKey key = kJoin && c.drop.state ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
   const float inv_w = 1.f / (float)width;
@@ -55,65 +49,67 @@ norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
   for (int64_t base = first - t.sub; base < c.rows; base += step) {      // (a warp's teams go on together)
     const int64_t r = base + t.sub;
     const bool live = r < c.rows;
-    zp_copy_wait(stages - 2);
+    zp_copy_wait(stages);
     if (!kAligned) t.sync();                   // others' pieces are there; the last row has been read
-    fetch(r + (stages - 1) * step, stage == 0 ? stages - 1 : stage - 1);
-    char *slot = ring + stage * A * p.slot + zp_row_place<T, kAligned>(src[0], r);
+    fetch(stage == 0 ? stages - 1 : stage - 1);
+    const char *const slot = ring + stage * A * p.slot;
+    const char *const x = slot + (kAligned ? 0 : sx.place), *const res = slot + p.slot + (kAligned ? 0 : sr.place);
+    sx.advance();
+    sr.advance();
     stage = stage + 1 == stages ? 0 : stage + 1;
     const int mine = live ? width : 0;
-    if constexpr (kJoin) {
-      uint32_t kept = 0xffffffffu;
-      if (c.drop.state) kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, live ? r : 0, width, bytes);
-      const char *res = slot - zp_row_place<T, kAligned>(src[0], r) + p.slot + zp_row_place<T, kAligned>(src[1], r);
-#pragma unroll
-      for (int i = 0; i < M; ++i) {
-        if (column(i, 0) >= mine) continue;
-        float v[V], q[V];
-        zp_read<T, kAligned>(t, slot, i, v);
-        zp_read<T, kAligned>(t, res, i, q);
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = q[k] + (kept >> (i * V + k) & 1 ? v[k] * c.drop.scale : 0.f);
-        zp_write<T, kAligned>(t, slot, i, v);          // rounded: what follows works on the sum as returned
-        zp_write<T, kAligned>(t, static_cast<T *>(c.sum) + r * c.width, i, v);
-      }
-    }
-    float s = 0.f;
+    uint32_t kept = 0xffffffffu;
+    if (kJoin && c.drop.state)
+      kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, live ? r : 0, width, bytes);
+    float v[E], s = 0.f;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
-      if (column(i, 0) >= mine) continue;
-      float v[V];
-      zp_read<T, kAligned>(t, slot, i, v);
+      float u[V] = {};
+      if (column(i, 0) < mine) {
+        zp_read<T, kAligned>(t, x, i, u);
+        if constexpr (kJoin) {
+          float q[V];
+          zp_read<T, kAligned>(t, res, i, q);
 #pragma unroll
-      for (int k = 0; k < V; ++k) s += v[k];
+          for (int k = 0; k < V; ++k)          // rounded: what follows works on the sum as it is returned
+            u[k] = zp_float(zp_rounded<T>(q[k] + (kept >> (i * V + k) & 1 ? u[k] * c.drop.scale : 0.f)));
+          zp_write<T, kAligned>(t, static_cast<T *>(c.sum) + r * c.width, i, u);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        v[i * V + k] = u[k];
+        s += u[k];
+      }
     }
     const float mean = t.sum(s, 0) * inv_w;
     float q = 0.f;
 #pragma unroll
-    for (int i = 0; i < M; ++i) {
-      if (column(i, 0) >= mine) continue;
-      float v[V];
-      zp_read<T, kAligned>(t, slot, i, v);
+    for (int i = 0; i < M; ++i)
+      if (column(i, 0) < mine) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) q += (v[k] - mean) * (v[k] - mean);
-    }
+        for (int k = 0; k < V; ++k) {
+          v[i * V + k] -= mean;
+          q += v[i * V + k] * v[i * V + k];
+        }
+      }
     const float rstd = rsqrtf(t.sum(q, 1) * inv_w + c.eps);
     T *const y = static_cast<T *>(c.y) + r * c.width;
 #pragma unroll
-    for (int i = 0; i < M; ++i) {
-      if (column(i, 0) >= mine) continue;
-      float v[V];
-      zp_read<T, kAligned>(t, slot, i, v);
+    for (int i = 0; i < M; ++i)
+      if (column(i, 0) < mine) {
+        float u[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float ww = kHeld ? w[i * V + k] : zp_param<T>(c.w, wide, column(i, k), 1.f);
-        const float bb = kHeld ? b[i * V + k] : zp_param<T>(c.b, wide, column(i, k), 0.f);
-        v[k] = (v[k] - mean) * rstd * ww + bb;
+        for (int k = 0; k < V; ++k) {
+          const float ww = kHeld ? w[kHeld ? i * V + k : 0] : zp_param<T>(c.w, wide, column(i, k), 1.f);
+          const float bb = kHeld ? b[kHeld ? i * V + k : 0] : zp_param<T>(c.b, wide, column(i, k), 0.f);
+          u[k] = v[i * V + k] * rstd * ww + bb;
+        }
+        zp_write<T, kAligned>(t, y, i, u);
       }
-      zp_write<T, kAligned>(t, y, i, v);
-    }
     if (c.mean && live && t.lane == 0) { c.mean[r] = mean; c.rstd[r] = rstd; }
   }
-  zp_copy_wait(0);
+  zp_copy_wait(2);
 }
 
 template <typename T, bool kAligned, int E, bool kJoin>
@@ -146,7 +142,7 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
                        (!c.res || (zp_piece_aligned(c.res, c.ldr, size) && zp_piece_aligned(c.sum, c.width, size))) &&
                        (!c.drop.state || c.width % 8 == 0);
   ZpTeamPlan p;
-  taken = zp_team_plan(c, aligned, c.res ? 2 : 1, 0, p);
+  taken = zp_team_plan(c, aligned, c.res ? 2 : 1, 0, 16, p);
   if (!taken) return ZP_OK;
   if (c.dtype == ZP_F32) return by_alignment<float>(c, p, st);
   if (c.dtype == ZP_F16) return by_alignment<__half>(c, p, st);
