@@ -75,10 +75,12 @@ dropout_pieces_kernel(int64_t groups, uint32_t per_row, const T *__restrict__ x,
 #pragma unroll
       for (int h = 0; h < kPieces; ++h) {
         if (p0 + 32 * (i + h) + lane >= pieces) continue;
-        float v[V];
+        float2 v[V / 2];
         zp_unpack<T>(in[i + h], v);
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = kept[h] >> k & 1 ? v[k] * drop.scale : 0.f;
+        for (int k = 0; k < V / 2; ++k)
+          v[k] = make_float2(kept[h] >> (2 * k) & 1 ? v[k].x * drop.scale : 0.f,
+                             kept[h] >> (2 * k + 1) & 1 ? v[k].y * drop.scale : 0.f);
         __stcs(reinterpret_cast<uint4 *>(y + to[i + h]), zp_pack<T>(v));
       }
     }

@@ -1,13 +1,16 @@
 // Operators over the rows of a matrix: what their kernels share.
 //
-// A row is worked on by a team of 2 to 512 threads, eight elements (or 16, or 32) to a thread; teams of a
-// warp or less add up by shuffles, larger ones through shared memory and a named barrier of their own.
-// Rows come in through a ring in shared memory that asynchronous copies keep filled several rows ahead: a
-// row of 128 to 4096 elements is 0.25 to 16 KB, and the 6.5 TB/s of the memory want some 40 KB in flight
-// on every SM, which registers do not hold beside the sums.
-//   aligned rows   a thread copies the 16-byte pieces that it works on itself: nobody waits for anybody
-//   other rows     the 16-byte pieces that the row lies in, whose they may be; a barrier, and every thread
-//                  reads its elements from wherever they fell
+// A row is worked on by a team of 2 to 512 threads, E elements to a thread in pieces of 16 bytes; a team
+// takes R rows at a time, so that what a row costs beside its elements (the joining of sums, barriers,
+// addresses) is shared.  Teams of a warp or less add up by shuffles, larger ones through shared memory and a
+// named barrier of their own.  Arithmetic on the elements goes by pairs (one instruction for two): these
+// kernels have 20 to 30 instruction slots for an element at the memory's speed, and spend 8 to 15.
+//
+// Rows come in through a ring in shared memory that asynchronous copies keep filled: the 6.5 TB/s of the
+// memory want some 40 KB in flight on every SM, which registers do not hold beside the sums.
+//   aligned rows   a thread copies the pieces that it works on itself: nobody waits for anybody
+//   other rows     the 16-byte pieces that the row lies in come as they are; after a barrier a thread puts
+//                  its pieces together from two of them, and results go the same way back
 #pragma once
 
 #include <cuda_bf16.h>
@@ -55,37 +58,39 @@ template <> __device__ __forceinline__ __nv_bfloat16 zp_rounded<__nv_bfloat16>(f
 
 template <typename T> constexpr int kZpVec = 16 / (int)sizeof(T);      // elements of a 16-byte piece
 
-// 16 bytes of T to floats and back
-template <typename T> __device__ __forceinline__ void zp_unpack(const uint4 &q, float (&v)[kZpVec<T>]) {
+// 16 bytes of T to pairs of floats and back
+template <typename T> __device__ __forceinline__ void zp_unpack(const uint4 &q, float2 (&v)[kZpVec<T> / 2]) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if constexpr (sizeof(T) == 4) {
-      v[k] = __uint_as_float(w[k]);
-    } else if constexpr (std::is_same<T, __half>::value) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
-      v[2 * k] = f.x; v[2 * k + 1] = f.y;
-    } else {
-      v[2 * k] = __uint_as_float(w[k] << 16);
-      v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+    for (int k = 0; k < 2; ++k) v[k] = make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (std::is_same<T, __half>::value)
+        v[k] = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+      else
+        v[k] = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xFFFF0000u));
     }
   }
 }
-template <typename T> __device__ __forceinline__ uint4 zp_pack(const float (&v)[kZpVec<T>]) {
-  uint32_t w[4];
+template <typename T> __device__ __forceinline__ uint4 zp_pack(const float2 (&v)[kZpVec<T> / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+  } else {
+    uint32_t w[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if constexpr (sizeof(T) == 4) {
-      w[k] = __float_as_uint(v[k]);
-    } else if constexpr (std::is_same<T, __half>::value) {
-      const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-      w[k] = *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-      w[k] = *reinterpret_cast<const uint32_t *>(&h);
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __float22half2_rn(v[k]);
+        w[k] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __nv_bfloat162 h = __float22bfloat162_rn(v[k]);
+        w[k] = *reinterpret_cast<const uint32_t *>(&h);
+      }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // element c of a parameter vector of type ZP_F32 (`wide`) or T
@@ -95,20 +100,46 @@ __device__ __forceinline__ float zp_param(const void *w, bool wide, int64_t c, f
   return wide ? static_cast<const float *>(w)[c] : zp_float(static_cast<const T *>(w)[c]);
 }
 
+// elements c .. c + V - 1 of one; vectors: they lie in aligned pieces of 16 bytes
+template <typename T>
+__device__ __forceinline__ void zp_params(const void *w, bool wide, bool vectors, int c, int width, float otherwise,
+                                          float2 (&v)[kZpVec<T> / 2]) {
+  constexpr int V = kZpVec<T>;
+  if (!w || c >= width) {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) v[k] = make_float2(otherwise, otherwise);
+  } else if (vectors && wide) {
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) {
+      const float4 q = reinterpret_cast<const float4 *>(static_cast<const float *>(w) + c)[k];
+      v[2 * k] = make_float2(q.x, q.y);
+      v[2 * k + 1] = make_float2(q.z, q.w);
+    }
+  } else if (vectors) {
+    zp_unpack<T>(*reinterpret_cast<const uint4 *>(static_cast<const T *>(w) + c), v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k)
+      v[k] = make_float2(c + 2 * k < width ? zp_param<T>(w, wide, c + 2 * k, 0.f) : otherwise,
+                         c + 2 * k + 1 < width ? zp_param<T>(w, wide, c + 2 * k + 1, 0.f) : otherwise);
+  }
+}
+
 // ---- teams ----------------------------------------------------------------------------------------
 
 constexpr int kZpTeamThreads = 512;            // of a block
+constexpr int kZpTeamWarps = kZpTeamThreads / 32;
 
 // Where a thread stands.  A "walker" is what goes through rows by itself: a warp, with one or several
-// teams in it, or a team of several warps.  It takes `per` rows at a time, one for each of its teams.
+// teams in it, or a team of several warps.
 struct ZpTeam {
   int size, lane;                              // threads of a team, this one's place in it
   int index;                                   // of the team in the block
-  int per, sub;                                // rows of a walker, this team's among them
+  int per, sub;                                // teams of a walker, this one among them
   int walker, walkers;
-  float2 *red;                                 // [2][warps of the block], for teams of several warps
+  float *red;                                  // [2][warps of the block][4], for teams of several warps
 
-  __device__ __forceinline__ ZpTeam(int team_size, float2 *red_) {
+  __device__ __forceinline__ ZpTeam(int team_size, float *red_) {
     size = team_size;
     const int tid = threadIdx.x, wide = size > 32 ? size : 32;
     lane = tid & (size - 1);
@@ -123,43 +154,59 @@ struct ZpTeam {
     if (size <= 32) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + index), "r"(size) : "memory");
   }
-  // sums over the team, the same in all of it; `turn` alternates from sum to sum (a buffer that is
-  // written again has been read by all: the other's barrier lies in between)
-  __device__ __forceinline__ float2 sum(float2 v, int turn) const {
+  // Sums of K values over the team, the same in all of it.  `turn` alternates from call to call (a buffer
+  // that is written again has been read by all: the other's barrier lies in between); `order`: what
+  // was read and written in shared memory before is ordered against what comes after.
+  // Over a warp, K values take 5 + K - 1 exchanges instead of 5 K: lanes send away the values that
+  // they will not add up further.
+  template <int K> __device__ __forceinline__ void sum(float (&v)[K], int turn, bool order) const {
+    static_assert(K == 1 || K == 2 || K == 4, "");
+    if (size < 32) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      if (o >= size) continue;
-      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+      for (int o = 8; o > 0; o >>= 1) {
+        if (o >= size) continue;
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+      }
+      if (order) __syncwarp();
+      return;
     }
-    if (size <= 32) return v;
-    float2 *at = red + (turn & 1) * (kZpTeamThreads / 32);
-    if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
-    sync();
-    const int n = size >> 5;                   // warps: each adds up all of them, in the same order
-    v = at[index * n + (threadIdx.x & (n - 1))];
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      if (o >= n) continue;
-      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    const int at = threadIdx.x & 31;
+    constexpr int kOwn = 32 / K;               // lanes that add up one value
+    float s;
+    if constexpr (K == 4) {
+      const bool hi = at & 16, up = at & 8;
+      const float a = (hi ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 16);
+      const float b = (hi ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 16);
+      s = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 8);
+    } else if constexpr (K == 2) {
+      const bool hi = at & 16;
+      s = (hi ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[1], 16);
+    } else {
+      s = v[0];
     }
-    return v;
-  }
-  __device__ __forceinline__ float sum(float v, int turn) const {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      if (o < size) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (size <= 32) return v;
-    float *at = reinterpret_cast<float *>(red + (turn & 1) * (kZpTeamThreads / 32));
-    if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
-    sync();
-    const int n = size >> 5;
-    v = at[index * n + (threadIdx.x & (n - 1))];
+    for (int o = kOwn / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (size > 32) {
+      float *const buf = red + (turn & 1) * (kZpTeamWarps * 4);
+      if (at % kOwn == 0) buf[(threadIdx.x >> 5) * K + at / kOwn] = s;
+      sync();
+      const int n = size >> 5, first = index * n;            // warps of the team
+      const float *from = buf + at / kOwn;
+      s = from[(first + (at % kOwn & (n - 1))) * K];
+      if (kOwn == 8 && n == 16) s += from[(first + at % kOwn + 8) * K];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1)
-      if (o < n) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+      for (int o = kOwn / 2; o > 0; o >>= 1)
+        if (o < n) s += __shfl_xor_sync(0xffffffffu, s, o);
+    } else if (order) {
+      __syncwarp();
+    }
+    if constexpr (K == 1) {
+      v[0] = s;
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, s, k * kOwn);
+    }
   }
 };
 
@@ -169,44 +216,43 @@ __device__ __forceinline__ void zp_copy16(uint32_t to, const void *from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void zp_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// until of this thread's latest groups at most `stages` - 2 are on their way (stages: 2 or 4)
+// until of this thread's latest groups at most `stages` - 2 are on their way (stages: 2, 3 or 4)
 __device__ __forceinline__ void zp_copy_wait(int stages) {
   if (stages == 4) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// One of the arrays that a ring brings in: the next row to fetch, and the addresses that may be read.
+// One of the arrays that a ring brings in: the first of the next rows to fetch, and the addresses that
+// may be read.
 struct ZpSource {
   const char *row, *begin, *end;
-  int64_t step;                                // bytes from a team's row to its next
-  int place, turn;                             // of the row that is worked on within 16 bytes; added per row
+  int64_t step, next;                          // bytes from a team's rows to its next ones, and between them
+  int place;                                   // within 16 bytes, of the rows that are worked on
   __device__ __forceinline__ ZpSource(const void *base, int64_t ld, int64_t rows, int64_t width, int size,
-                                      int64_t first, int64_t rows_per_step) {
+                                      int64_t first, int64_t rows_per_step, int per) {
     begin = static_cast<const char *>(base);
     end = begin + ((rows - 1) * ld + width) * size;
     row = begin + first * ld * size;
     step = rows_per_step * ld * size;
+    next = per * ld * size;
     place = (int)(reinterpret_cast<uintptr_t>(row) & 15);
-    turn = (int)(step & 15);
   }
-  __device__ __forceinline__ void advance() { place = (place + turn) & 15; }
+  __device__ __forceinline__ int place_of(int j) const { return (place + j * (int)(next & 15)) & 15; }
+  __device__ __forceinline__ void advance() { place = (place + (int)(step & 15)) & 15; }
 };
 
-// The next row of `width` elements of T into a slot.  kAligned: element c goes to byte c * sizeof(T), each
-// thread copies its own.  Else the row keeps its place within 16 bytes.
-template <typename T, bool kAligned, int E>
-__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, char *slot, ZpSource &s, bool live, int width) {
-  const char *const row = s.row;
-  s.row += s.step;
-  if (!live) return;
+// A row of `width` elements of T into a slot.  kAligned: element c goes to byte c * sizeof(T), each thread
+// copies its own pieces.  Else the row keeps its place within 16 bytes.
+template <typename T, bool kAligned, int M>
+__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, char *slot, const ZpSource &s, const char *row,
+                                             int width) {
   if constexpr (kAligned) {
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot) + 16 * t.lane;
     const char *const from = row + 16 * t.lane;
 #pragma unroll
-    for (int i = 0; i < E / kZpVec<T>; ++i) {
-      const int piece = t.lane + i * t.size;
-      if (piece * kZpVec<T> < width) zp_copy16(to + 16 * i * t.size, from + 16 * i * t.size);
-    }
+    for (int i = 0; i < M; ++i)
+      if ((t.lane + i * t.size) * kZpVec<T> < width) zp_copy16(to + 16 * i * t.size, from + 16 * i * t.size);
   } else {
     const char *from = reinterpret_cast<const char *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
     const char *end = row + width * (int)sizeof(T);
@@ -223,38 +269,94 @@ __device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, char *slot, ZpSour
   }
 }
 
-// A thread's V elements number i of a row in a slot (kAligned: a piece of 16 bytes, else one element)
-template <typename T, bool kAligned> constexpr int kZpStep = kAligned ? kZpVec<T> : 1;
-template <typename T, bool kAligned>
-__device__ __forceinline__ void zp_read(const ZpTeam &t, const char *slot, int i,
-                                        float (&v)[kZpStep<T, kAligned>]) {
-  if constexpr (kAligned) zp_unpack<T>(*reinterpret_cast<const uint4 *>(slot + 16 * (t.lane + i * t.size)), v);
-  else v[0] = zp_float(*reinterpret_cast<const T *>(slot + sizeof(T) * (t.lane + i * t.size)));
+// the 16 bytes of shared memory that begin `place` (0 .. 15, a multiple of kSize) behind 16-byte piece q
+template <int kSize> __device__ __forceinline__ uint4 zp_read_between(const char *slot, int q, int place) {
+  const uint4 a = *reinterpret_cast<const uint4 *>(slot + 16 * q), b = *reinterpret_cast<const uint4 *>(slot + 16 * q + 16);
+  uint32_t w[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
+  const bool two = place & 8, one = place & 4;
+  uint32_t x[6], y[5];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) x[k] = two ? w[k + 2] : w[k];
+  x[5] = two ? b.w : w[5];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) y[k] = one ? x[k + 1] : x[k];
+  if constexpr (kSize == 2) {
+    const int half = (place & 2) * 8;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = __funnelshift_r(y[k], y[k + 1], half);
+  }
+  return make_uint4(y[0], y[1], y[2], y[3]);
 }
-// ... and to memory (or back to the slot): `row` is the address of the row's first element
+
+// zeroes what of piece q lies past the row's end
+template <typename T> __device__ __forceinline__ void zp_cut(int q, int width, float2 (&v)[kZpVec<T> / 2]) {
+  const int left = width - q * kZpVec<T>;
+  if (left >= kZpVec<T>) return;
+#pragma unroll
+  for (int k = 0; k < kZpVec<T> / 2; ++k) {
+    if (2 * k >= left) v[k].x = 0.f;
+    if (2 * k + 1 >= left) v[k].y = 0.f;
+  }
+}
+// Piece number i of a thread, of a row in a slot.  Elements past the row's end are zero.
 template <typename T, bool kAligned>
-__device__ __forceinline__ void zp_write(const ZpTeam &t, void *row, int i, const float (&v)[kZpStep<T, kAligned>]) {
-  if constexpr (kAligned) static_cast<uint4 *>(row)[t.lane + i * t.size] = zp_pack<T>(v);
-  else static_cast<T *>(row)[t.lane + i * t.size] = zp_rounded<T>(v[0]);
+__device__ __forceinline__ void zp_read(const ZpTeam &t, const char *slot, int place, int i, int width,
+                                        float2 (&v)[kZpVec<T> / 2]) {
+  const int q = t.lane + i * t.size;
+  if constexpr (kAligned) {
+    zp_unpack<T>(*reinterpret_cast<const uint4 *>(slot + 16 * q), v);
+  } else {
+    zp_unpack<T>(zp_read_between<sizeof(T)>(slot, q, place), v);
+    zp_cut<T>(q, width, v);
+  }
+}
+// Results: aligned rows straight to memory; others into a slot, 16 bytes from its start, from where
+// zp_store_row takes them once the whole team has written.
+template <typename T, bool kAligned>
+__device__ __forceinline__ void zp_write(const ZpTeam &t, char *row, char *slot, int i,
+                                         const float2 (&v)[kZpVec<T> / 2]) {
+  const int q = t.lane + i * t.size;
+  if constexpr (kAligned) reinterpret_cast<uint4 *>(row)[q] = zp_pack<T>(v);
+  else reinterpret_cast<uint4 *>(slot)[q + 1] = zp_pack<T>(v);
+}
+template <typename T>
+__device__ __forceinline__ void zp_store_row(const ZpTeam &t, char *row, const char *slot, int width) {
+  const int place = (int)(reinterpret_cast<uintptr_t>(row) & 15), bytes = width * (int)sizeof(T);
+  char *const at = row - place;                // (a piece that begins before the row is not stored whole)
+  const int back = place ? 0 : 1;
+  for (int q = t.lane; 16 * q < place + bytes; q += t.size) {
+    const uint4 v = zp_read_between<sizeof(T)>(slot, q + back, (16 - place) & 15);
+    if (16 * q >= place && 16 * q + 16 <= place + bytes) {
+      *reinterpret_cast<uint4 *>(at + 16 * q) = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < kZpVec<T>; ++k) {
+        const int b = 16 * q + k * (int)sizeof(T);
+        if (b < place || b >= place + bytes) continue;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t *>(at + b) = w[k];
+        else *reinterpret_cast<uint16_t *>(at + b) = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
+      }
+    }
+  }
 }
 
 // ---- which of a thread's elements are kept ----------------------------------------------------------
-// Bit e of the result: the thread's element e (of E, V of them side by side) of row r is kept.
+// Bit i * V + k of the result: element k of the thread's piece i of row r is kept.
 //   aligned, 16-bit   a piece is one counter's eight elements
 //   aligned, fp32     a piece is half of them: of two neighbours each works out one of two counters, and
 //                     they swap
 //   other rows        the team works out the row's counters, eight bits each into `bytes`
-//                     [width / 8 + 2], and every thread looks up its own
+//                     [width / 8 + 3], and every thread looks up its own
 // All threads of a warp come here together.
 template <typename T, bool kAligned, int E>
 __device__ __forceinline__ uint32_t zp_kept_bits(const ZpTeam &t, const ZpPhiloxKey &key, uint32_t threshold,
                                                  int64_t r, int width, uint8_t *bytes) {
   uint32_t bits = 0;
   if constexpr (kAligned && sizeof(T) == 2) {
-    const uint64_t first = (uint64_t)r * (uint32_t)(width / 8);
+    const uint64_t first = (uint64_t)r * (uint32_t)(width / 8) + t.lane;
 #pragma unroll
-    for (int i = 0; i < E / 8; ++i)
-      bits |= zp_philox_kept(key, first + t.lane + i * t.size, threshold) << (8 * i);
+    for (int i = 0; i < E / 8; ++i) bits |= zp_philox_kept(key, first + i * t.size, threshold) << (8 * i);
   } else if constexpr (kAligned) {
     const uint64_t first = (uint64_t)r * (uint32_t)(width / 8);
     const int odd = t.lane & 1;
@@ -267,15 +369,19 @@ __device__ __forceinline__ uint32_t zp_kept_bits(const ZpTeam &t, const ZpPhilox
       bits |= (lo | hi << 4) << (8 * i);
     }
   } else {
+    constexpr int V = kZpVec<T>;
     const uint64_t e0 = (uint64_t)r * (uint64_t)width;
     const int groups = (int)((e0 + width - 1) / 8 - e0 / 8) + 1, place = (int)(e0 & 7);
     t.sync();                                  // the last row's have been looked up
     for (int g = t.lane; g < groups; g += t.size) bytes[g] = (uint8_t)zp_philox_kept(key, e0 / 8 + g, threshold);
     t.sync();
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int c = t.lane + i * t.size;
-      if (c < width) bits |= (uint32_t)(bytes[(place + c) >> 3] >> ((place + c) & 7) & 1) << i;
+    for (int i = 0; i < E / V; ++i) {
+      const int c = (t.lane + i * t.size) * V, at = (place + c) >> 3;
+      if (c < width) {
+        const uint32_t two = bytes[at] | (uint32_t)bytes[at + 1] << 8;
+        bits |= (two >> ((place + c) & 7) & ((1u << V) - 1)) << (i * V);
+      }
     }
   }
   return bits;
@@ -283,40 +389,38 @@ __device__ __forceinline__ uint32_t zp_kept_bits(const ZpTeam &t, const ZpPhilox
 
 // ---- launches ---------------------------------------------------------------------------------------
 
-// How a call's rows are shared out: elements per thread, the team's size, whether pieces of 16 bytes are
-// aligned, and the ring's sizes.
+// How a call's rows are shared out: elements per thread and rows at a time, the team's size, whether pieces
+// of 16 bytes are aligned (of the rows, and of weight and bias), and the ring's sizes.
 struct ZpTeamPlan {
-  int team, elements;
-  bool aligned;
+  int team, elements, rows;
+  bool aligned, vectors;
   int slot, bytes, stages;                     // bytes of a slot, of the counters' bits of a team
   size_t smem;
   unsigned blocks;
 };
 // `arrays` come in per row; `last_per_element`: bytes of shared memory per element of a block's teams that
-// the kernel needs when the ring is done with; `most`: elements of a thread where there are rows enough.
-// False: the rows are too wide.
-inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, size_t last_per_element, int most,
-                         ZpTeamPlan &p) {
+// the kernel needs when the ring is done with.  False: this does not fit.
+inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, size_t last_per_element, int elements,
+                         int rows, ZpTeamPlan &p) {
   const int64_t size = c.dtype == ZP_F32 ? 4 : 2;
-  if (c.width > kZpTeamThreads * 32) return false;
+  if (c.width > (int64_t)kZpTeamThreads * elements) return false;
   p.aligned = aligned;
-  for (p.elements = 8; p.elements < 32; p.elements *= 2) {
-    if (c.width > (int64_t)kZpTeamThreads * p.elements) continue;
-    if (p.elements >= most || c.rows * c.width < (int64_t)148 * kZpTeamThreads * 2 * p.elements) break;
-  }
-  const int64_t need = zp_ceil_div(c.width, p.elements);
+  p.vectors = c.width % (16 / size) == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0 &&
+              reinterpret_cast<uintptr_t>(c.b) % 16 == 0;
+  p.elements = elements;
+  p.rows = rows;
+  const int64_t need = zp_ceil_div(c.width, elements);
   for (p.team = 2; p.team < need; p.team *= 2) {}
   const int teams = kZpTeamThreads / p.team;
-  p.slot = (int)zp_align_up((size_t)(p.team * p.elements * size) + (aligned ? 0 : 16), 16);
-  p.bytes = aligned || !c.drop.state ? 0 : (int)zp_align_up((size_t)c.width / 8 + 2, 16);
-  const size_t red = 2 * sizeof(float2) * (kZpTeamThreads / 32), fixed = red + (size_t)p.bytes * teams;
-  const size_t last = last_per_element * kZpTeamThreads * p.elements;
-  const size_t stage = (size_t)arrays * p.slot * teams;
-  const size_t room = 226 * 1024;
-  p.stages = fixed + 4 * stage <= room ? 4 : 2;
+  p.slot = (int)(p.team * elements * size) + (aligned ? 0 : 48);
+  p.bytes = aligned || !c.drop.state ? 0 : (int)zp_align_up((size_t)c.width / 8 + 3, 16);
+  const size_t red = sizeof(float) * 2 * 4 * kZpTeamWarps, fixed = red + (size_t)p.bytes * teams;
+  const size_t last = last_per_element * kZpTeamThreads * elements, room = 226 * 1024;
+  const size_t stage = (size_t)arrays * rows * p.slot * teams;
+  p.stages = fixed + 4 * stage <= room ? 4 : fixed + 3 * stage <= room ? 3 : 2;
   if (fixed + p.stages * stage > room || fixed + last > room) return false;
   p.smem = fixed + (p.stages * stage > last ? p.stages * stage : last);
-  const int64_t units = zp_ceil_div(c.rows, p.team < 32 ? 32 / p.team : 1);
+  const int64_t units = zp_ceil_div(c.rows, rows * (p.team < 32 ? 32 / p.team : 1));
   p.blocks = (unsigned)(units < 148 ? units : 148);
   return true;
 }

@@ -1,136 +1,179 @@
 // Forward of the layer norm over rows, alone and behind a residual sum with dropout.
 //
-// Memory bound: a row is read once and the results are written once; between lie about ten instructions
-// per element (and eight for the random bits).  Mean and variance take two passes over the row in shared
-// memory, the variance from differences to the mean: sums of squares would lose a mean that is large
-// against the spread.
+// Memory bound: a row is read once and the results are written once.  Mean and variance take two passes
+// over the row in registers, the variance from differences to the mean: sums of squares would lose a mean
+// that is large against the spread.
 #include "zp_rowwise.cuh"
 
 namespace {
 
-template <typename T, bool kAligned, int E, bool kJoin>
+// E elements of a thread in each of R rows at a time
+template <typename T, bool kAligned, int E, int R, bool kJoin>
 __global__ void __launch_bounds__(kZpTeamThreads, 1)
 norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
   zp_after_previous();
-  constexpr int V = kZpStep<T, kAligned>, M = E / V, A = kJoin ? 2 : 1;
+  constexpr int V = kZpVec<T>, H = V / 2, M = E / V, A = kJoin ? 2 : 1;
+  constexpr bool kHeld = E <= 16;              // weight and bias stay in registers
   extern __shared__ __align__(16) char smem[];
-  const ZpTeam t(p.team, reinterpret_cast<float2 *>(smem));
+  const ZpTeam t(p.team, reinterpret_cast<float *>(smem));
   const int width = (int)c.width, teams = kZpTeamThreads / p.team, stages = p.stages;
-  char *const after_red = smem + 2 * sizeof(float2) * (kZpTeamThreads / 32);
+  char *const after_red = smem + sizeof(float) * 2 * 4 * kZpTeamWarps;
   uint8_t *const bytes = reinterpret_cast<uint8_t *>(after_red) + t.index * p.bytes;
-  char *const ring = after_red + p.bytes * teams + (size_t)t.index * stages * A * p.slot;
-  const int64_t step = (int64_t)gridDim.x * t.walkers * t.per;
-  const int64_t first = ((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per + t.sub;
-  ZpSource sx(c.x, c.ldx, c.rows, c.width, sizeof(T), first, step);
-  ZpSource sr(c.res, c.ldr, c.rows, c.width, sizeof(T), first, step);
+  char *const ring = after_red + p.bytes * teams + (size_t)t.index * stages * A * R * p.slot;
+  // a walker takes R rows of each of its teams, its teams' side by side; rows of a team are `per` apart
+  const int64_t step = (int64_t)gridDim.x * t.walkers * t.per * R;
+  const int64_t first = ((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per * R + t.sub;
+  ZpSource sx(c.x, c.ldx, c.rows, c.width, sizeof(T), first, step, t.per);
+  ZpSource sr(c.res, c.ldr, c.rows, c.width, sizeof(T), first, step, t.per);
   int64_t coming = first;
   auto fetch = [&](int stage) {
-    char *const to = ring + stage * A * p.slot;
-    zp_fetch_row<T, kAligned, E>(t, to, sx, coming < c.rows, width);
-    if (kJoin) zp_fetch_row<T, kAligned, E>(t, to + p.slot, sr, coming < c.rows, width);
+    char *to = ring + stage * A * R * p.slot;
+#pragma unroll
+    for (int j = 0; j < R; ++j, to += A * p.slot) {
+      if (coming + j * t.per >= c.rows) continue;
+      zp_fetch_row<T, kAligned, M>(t, to, sx, sx.row + j * sx.next, width);
+      if (kJoin) zp_fetch_row<T, kAligned, M>(t, to + p.slot, sr, sr.row + j * sr.next, width);
+    }
+    sx.row += sx.step;
+    sr.row += sr.step;
     coming += step;
     zp_copy_commit();
   };
   for (int s = 0; s < stages - 1; ++s) fetch(s);
 
   const bool wide = c.param_dtype == ZP_F32;
-  auto column = [&](int i, int k) { return (t.lane + i * t.size) * V + k; };
-  constexpr bool kHeld = E <= 16;              // weight and bias stay in registers
-  float w[kHeld ? E : 1], b[kHeld ? E : 1];
+  auto column = [&](int i) { return (t.lane + i * t.size) * V; };
+  float2 w[kHeld ? M : 1][H], b[kHeld ? M : 1][H];
 #pragma unroll
-  for (int e = 0; e < (kHeld ? E : 0); ++e) {
-    const int col = column(e / V, e % V);
-    w[e] = col < width ? zp_param<T>(c.w, wide, col, 1.f) : 0.f;
-    b[e] = col < width ? zp_param<T>(c.b, wide, col, 0.f) : 0.f;
+  for (int i = 0; i < (kHeld ? M : 0); ++i) {
+    zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, w[i]);
+    zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, b[i]);
   }
   const ZpPhiloxKey key = kJoin && c.drop.state ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
   const float inv_w = 1.f / (float)width;
+  const int64_t row_bytes = c.width * (int64_t)sizeof(T);
   int stage = 0;
-  for (int64_t base = first - t.sub; base < c.rows; base += step) {      // (a warp's teams go on together)
-    const int64_t r = base + t.sub;
-    const bool live = r < c.rows;
+  for (int64_t r0 = first; r0 - t.sub < c.rows; r0 += step) {        // (a warp's teams go on together)
     zp_copy_wait(stages);
-    if (!kAligned) t.sync();                   // others' pieces are there; the last row has been read
+    if (!kAligned) t.sync();                   // others' pieces are there; the last rows have been read
     fetch(stage == 0 ? stages - 1 : stage - 1);
-    const char *const slot = ring + stage * A * p.slot;
-    const char *const x = slot + (kAligned ? 0 : sx.place), *const res = slot + p.slot + (kAligned ? 0 : sr.place);
-    sx.advance();
-    sr.advance();
+    char *const slots = ring + stage * A * R * p.slot;
     stage = stage + 1 == stages ? 0 : stage + 1;
-    const int mine = live ? width : 0;
-    uint32_t kept = 0xffffffffu;
-    if (kJoin && c.drop.state)
-      kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, live ? r : 0, width, bytes);
-    float v[E], s = 0.f;
+    float2 v[R][M][H];
+    float s[R];
+    int mine[R];
 #pragma unroll
-    for (int i = 0; i < M; ++i) {
-      float u[V] = {};
-      if (column(i, 0) < mine) {
-        zp_read<T, kAligned>(t, x, i, u);
+    for (int j = 0; j < R; ++j) {
+      const int64_t r = r0 + j * t.per;
+      mine[j] = r < c.rows ? width : 0;
+      char *const x = slots + j * A * p.slot, *const res = x + p.slot;
+      uint32_t kept = 0xffffffffu;
+      if (kJoin && c.drop.state)
+        kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, mine[j] ? r : 0, width, bytes);
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) v[j][i][k] = make_float2(0.f, 0.f);
+        if (column(i) >= mine[j]) continue;
+        zp_read<T, kAligned>(t, x, sx.place_of(j), i, width, v[j][i]);
         if constexpr (kJoin) {
-          float q[V];
-          zp_read<T, kAligned>(t, res, i, q);
+          float2 q[H];
+          zp_read<T, kAligned>(t, res, sr.place_of(j), i, width, q);
 #pragma unroll
-          for (int k = 0; k < V; ++k)          // rounded: what follows works on the sum as it is returned
-            u[k] = zp_float(zp_rounded<T>(q[k] + (kept >> (i * V + k) & 1 ? u[k] * c.drop.scale : 0.f)));
-          zp_write<T, kAligned>(t, static_cast<T *>(c.sum) + r * c.width, i, u);
+          for (int k = 0; k < H; ++k) {
+            const uint32_t two = kept >> (i * V + 2 * k);
+            const float2 f = make_float2(two & 1 ? v[j][i][k].x * c.drop.scale : 0.f,
+                                         two & 2 ? v[j][i][k].y * c.drop.scale : 0.f);
+            v[j][i][k] = __fadd2_rn(q[k], f);
+          }
+          // rounded: what follows works on the sum as it is returned
+          const uint4 packed = zp_pack<T>(v[j][i]);
+          if (kAligned)
+            reinterpret_cast<uint4 *>(static_cast<char *>(c.sum) + r * row_bytes)[t.lane + i * t.size] = packed;
+          zp_unpack<T>(packed, v[j][i]);
         }
-      }
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        v[i * V + k] = u[k];
-        s += u[k];
+        for (int k = 0; k < H; ++k) sum = __fadd2_rn(sum, v[j][i][k]);
+      }
+      s[j] = sum.x + sum.y;
+    }
+    t.sum(s, 0, !kAligned);
+    float q[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      s[j] *= inv_w;
+      float2 sq = make_float2(0.f, 0.f);
+      const float2 minus = make_float2(-s[j], -s[j]);
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        if (column(i) >= mine[j]) continue;
+        if constexpr (kJoin && !kAligned)      // (the team has read all of this slot)
+          zp_write<T, kAligned>(t, nullptr, slots + j * A * p.slot, i, v[j][i]);
+#pragma unroll
+        for (int k = 0; k < H; ++k) v[j][i][k] = __fadd2_rn(v[j][i][k], minus);
+        if constexpr (!kAligned) zp_cut<T>(t.lane + i * t.size, width, v[j][i]);
+#pragma unroll
+        for (int k = 0; k < H; ++k) sq = __ffma2_rn(v[j][i][k], v[j][i][k], sq);
+      }
+      q[j] = sq.x + sq.y;
+    }
+    t.sum(q, 1, !kAligned);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int64_t r = r0 + j * t.per;
+      const float rstd = rsqrtf(q[j] * inv_w + c.eps);
+      const float2 both = make_float2(rstd, rstd);
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        if (column(i) >= mine[j]) continue;
+        float2 ww[H], bb[H];
+        if constexpr (!kHeld) {
+          zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, ww);
+          zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, bb);
+        }
+#pragma unroll
+        for (int k = 0; k < H; ++k)
+          v[j][i][k] = __ffma2_rn(__fmul2_rn(v[j][i][k], both), kHeld ? w[kHeld ? i : 0][k] : ww[k],
+                                  kHeld ? b[kHeld ? i : 0][k] : bb[k]);
+        zp_write<T, kAligned>(t, static_cast<char *>(c.y) + r * row_bytes, slots + (j * A + A - 1) * p.slot, i, v[j][i]);
+      }
+      if (c.mean && mine[j] && t.lane == 0) { c.mean[r] = s[j]; c.rstd[r] = rstd; }
+    }
+    if constexpr (!kAligned) {
+      t.sync();
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int64_t r = r0 + j * t.per;
+        if (!mine[j]) continue;
+        zp_store_row<T>(t, static_cast<char *>(c.y) + r * row_bytes, slots + (j * A + A - 1) * p.slot, width);
+        if (kJoin) zp_store_row<T>(t, static_cast<char *>(c.sum) + r * row_bytes, slots + j * A * p.slot, width);
       }
     }
-    const float mean = t.sum(s, 0) * inv_w;
-    float q = 0.f;
-#pragma unroll
-    for (int i = 0; i < M; ++i)
-      if (column(i, 0) < mine) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          v[i * V + k] -= mean;
-          q += v[i * V + k] * v[i * V + k];
-        }
-      }
-    const float rstd = rsqrtf(t.sum(q, 1) * inv_w + c.eps);
-    T *const y = static_cast<T *>(c.y) + r * c.width;
-#pragma unroll
-    for (int i = 0; i < M; ++i)
-      if (column(i, 0) < mine) {
-        float u[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float ww = kHeld ? w[kHeld ? i * V + k : 0] : zp_param<T>(c.w, wide, column(i, k), 1.f);
-          const float bb = kHeld ? b[kHeld ? i * V + k : 0] : zp_param<T>(c.b, wide, column(i, k), 0.f);
-          u[k] = v[i * V + k] * rstd * ww + bb;
-        }
-        zp_write<T, kAligned>(t, y, i, u);
-      }
-    if (c.mean && live && t.lane == 0) { c.mean[r] = mean; c.rstd[r] = rstd; }
+    sx.advance();
+    sr.advance();
   }
   zp_copy_wait(2);
 }
 
-template <typename T, bool kAligned, int E, bool kJoin>
+template <typename T, bool kAligned, int E, int R, bool kJoin>
 int launch(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
   static ZpSmemOptIn opt_in;
-  if (int rc = zp_ensure_smem(norm_fwd_team_kernel<T, kAligned, E, kJoin>, p.smem, opt_in)) return rc;
-  zp_launch(norm_fwd_team_kernel<T, kAligned, E, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
+  if (int rc = zp_ensure_smem(norm_fwd_team_kernel<T, kAligned, E, R, kJoin>, p.smem, opt_in)) return rc;
+  zp_launch(norm_fwd_team_kernel<T, kAligned, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
   ZP_LAUNCH_CHECK("norm_fwd_team_kernel");
   return ZP_OK;
 }
-template <typename T, bool kAligned, int E>
-int by_join(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  return c.res ? launch<T, kAligned, E, true>(c, p, st) : launch<T, kAligned, E, false>(c, p, st);
+template <typename T, bool kAligned, bool kJoin>
+int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+  if (p.elements == 8) return p.rows == 1 ? launch<T, kAligned, 8, 1, kJoin>(c, p, st) : launch<T, kAligned, 8, 2, kJoin>(c, p, st);
+  if (p.elements == 16)
+    return p.rows == 1 ? launch<T, kAligned, 16, 1, kJoin>(c, p, st) : launch<T, kAligned, 16, 2, kJoin>(c, p, st);
+  return launch<T, kAligned, 32, 1, kJoin>(c, p, st);
 }
-template <typename T, bool kAligned> int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  return p.elements == 8    ? by_join<T, kAligned, 8>(c, p, st)
-         : p.elements == 16 ? by_join<T, kAligned, 16>(c, p, st)
-                            : by_join<T, kAligned, 32>(c, p, st);
-}
-template <typename T> int by_alignment(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  return p.aligned ? by_elements<T, true>(c, p, st) : by_elements<T, false>(c, p, st);
+template <typename T> int by_kind(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+  if (c.res) return p.aligned ? by_elements<T, true, true>(c, p, st) : by_elements<T, false, true>(c, p, st);
+  return p.aligned ? by_elements<T, true, false>(c, p, st) : by_elements<T, false, false>(c, p, st);
 }
 
 }  // namespace
@@ -138,13 +181,21 @@ template <typename T> int by_alignment(const ZpNormCall &c, const ZpTeamPlan &p,
 int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
   const size_t size = c.dtype == ZP_F32 ? 4 : 2;
   // (results lie row behind row; the counters of dropout go by eight elements)
-  const bool aligned = (c.width * size) % 16 == 0 && zp_piece_aligned(c.x, c.ldx, size) && zp_piece_aligned(c.y, c.width, size) &&
+  const bool aligned = (c.width * size) % 16 == 0 && zp_piece_aligned(c.x, c.ldx, size) &&
+                       zp_piece_aligned(c.y, c.width, size) &&
                        (!c.res || (zp_piece_aligned(c.res, c.ldr, size) && zp_piece_aligned(c.sum, c.width, size))) &&
                        (!c.drop.state || c.width % 8 == 0);
+  // the more elements a thread has, the less the rest of a row's work weighs; few rows are spread over
+  // more threads instead
+  const int64_t n = c.rows * c.width, threads = (int64_t)148 * kZpTeamThreads;
+  const int arrays = c.res ? 2 : 1;
   ZpTeamPlan p;
-  taken = zp_team_plan(c, aligned, c.res ? 2 : 1, 0, 16, p);
+  taken = (n >= threads * 64 && zp_team_plan(c, aligned, arrays, 0, 16, 2, p)) ||
+          (n >= threads * 32 && zp_team_plan(c, aligned, arrays, 0, 8, 2, p)) ||
+          zp_team_plan(c, aligned, arrays, 0, 8, 1, p) || zp_team_plan(c, aligned, arrays, 0, 16, 1, p) ||
+          zp_team_plan(c, aligned, arrays, 0, 32, 1, p);
   if (!taken) return ZP_OK;
-  if (c.dtype == ZP_F32) return by_alignment<float>(c, p, st);
-  if (c.dtype == ZP_F16) return by_alignment<__half>(c, p, st);
-  return by_alignment<__nv_bfloat16>(c, p, st);
+  if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);
+  if (c.dtype == ZP_F16) return by_kind<__half>(c, p, st);
+  return by_kind<__nv_bfloat16>(c, p, st);
 }
