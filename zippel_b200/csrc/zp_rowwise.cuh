@@ -223,63 +223,85 @@ __device__ __forceinline__ void zp_copy_wait(int stages) {
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// One of the arrays that a ring brings in: the first of the next rows to fetch, and the addresses that
-// may be read.
-struct ZpSource {
+__device__ __forceinline__ uint32_t zp_shared(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint4 zp_lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 zp_lds8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ void zp_sts16(uint32_t at, const uint4 &v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// One of the arrays that a ring brings in: the first of the next rows to fetch (and, in aligned arrays, this
+// thread's first piece of it), and the addresses that may be read.
+template <bool kAligned> struct ZpSource {
   const char *row, *begin, *end;
-  int64_t step, next;                          // bytes from a team's rows to its next ones, and between them
-  int place;                                   // within 16 bytes, of the rows that are worked on
-  __device__ __forceinline__ ZpSource(const void *base, int64_t ld, int64_t rows, int64_t width, int size,
-                                      int64_t first, int64_t rows_per_step, int per) {
+  int64_t step, next;                          // bytes from a team's rows to its next ones, and from row to row
+  int place;                                   // within 16 bytes, of the first of the rows that are worked on
+  __device__ __forceinline__ ZpSource(const ZpTeam &t, const void *base, int64_t ld, int64_t rows, int64_t width,
+                                      int size, int64_t first, int64_t rows_per_step) {
     begin = static_cast<const char *>(base);
     end = begin + ((rows - 1) * ld + width) * size;
-    row = begin + first * ld * size;
+    row = begin + first * ld * size + (kAligned ? 16 * t.lane : 0);
     step = rows_per_step * ld * size;
-    next = per * ld * size;
-    place = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+    next = ld * size;
+    place = kAligned ? 0 : (int)(reinterpret_cast<uintptr_t>(row) & 15);
   }
-  __device__ __forceinline__ int place_of(int j) const { return (place + j * (int)(next & 15)) & 15; }
-  __device__ __forceinline__ void advance() { place = (place + (int)(step & 15)) & 15; }
+  __device__ __forceinline__ int place_of(int j) const {
+    return kAligned ? 0 : (place + j * (int)(next & 15)) & 15;
+  }
+  __device__ __forceinline__ void advance() {
+    if (!kAligned) place = (place + (int)(step & 15)) & 15;
+  }
 };
 
-// A row of `width` elements of T into a slot.  kAligned: element c goes to byte c * sizeof(T), each thread
-// copies its own pieces.  Else the row keeps its place within 16 bytes.
-template <typename T, bool kAligned, int M>
-__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, char *slot, const ZpSource &s, const char *row,
+// Row j of the next rows, `width` elements of T, into a slot.  kAligned: element c goes to byte
+// c * sizeof(T), each thread copies its own pieces (kFull: it has them all).  Else the row keeps its place
+// within 16 bytes.
+template <typename T, bool kAligned, bool kFull, int M>
+__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, uint32_t slot, const ZpSource<kAligned> &s, int j,
                                              int width) {
+  const char *const row = j ? s.row + j * s.next : s.row;
   if constexpr (kAligned) {
-    const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot) + 16 * t.lane;
-    const char *const from = row + 16 * t.lane;
+    const uint32_t to = slot + 16 * t.lane;
 #pragma unroll
     for (int i = 0; i < M; ++i)
-      if ((t.lane + i * t.size) * kZpVec<T> < width) zp_copy16(to + 16 * i * t.size, from + 16 * i * t.size);
+      if (kFull || (t.lane + i * t.size) * kZpVec<T> < width) zp_copy16(to + 16 * i * t.size, row + 16 * i * t.size);
   } else {
-    const char *from = reinterpret_cast<const char *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15);
-    const char *end = row + width * (int)sizeof(T);
-    for (const char *p = from + 16 * t.lane; p < end; p += 16 * t.size) {
-      char *to = slot + (p - from);
-      if (p >= s.begin && p + 16 <= s.end) {
-        zp_copy16((uint32_t)__cvta_generic_to_shared(to), p);
-      } else {                                 // the ends of the array: what lies outside is not read
-        for (int k = 0; k < 16; k += sizeof(T))
-          if (p + k >= row && p + k < end)
-            *reinterpret_cast<T *>(to + k) = *reinterpret_cast<const T *>(p + k);
+    const int place = (int)(reinterpret_cast<uintptr_t>(row) & 15), span = place + width * (int)sizeof(T);
+    const char *const from = row - place;
+    if (from >= s.begin && from + ((span + 15) & ~15) <= s.end) {
+#pragma unroll
+      for (int i = 0; i <= M; ++i) {
+        const int at = 16 * (t.lane + i * t.size);
+        if (at < span) zp_copy16(slot + at, from + at);
+      }
+    } else {                                   // the ends of the array: what lies outside is not read
+      for (int c = t.lane; c < width; c += t.size) {
+        const uint32_t to = slot + place + c * (int)sizeof(T);
+        if constexpr (sizeof(T) == 4)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(reinterpret_cast<const uint32_t *>(row)[c]) : "memory");
+        else
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"(reinterpret_cast<const uint16_t *>(row)[c]) : "memory");
       }
     }
   }
 }
 
-// the 16 bytes of shared memory that begin `place` (0 .. 15, a multiple of kSize) behind 16-byte piece q
-template <int kSize> __device__ __forceinline__ uint4 zp_read_between(const char *slot, int q, int place) {
-  const uint4 a = *reinterpret_cast<const uint4 *>(slot + 16 * q), b = *reinterpret_cast<const uint4 *>(slot + 16 * q + 16);
-  uint32_t w[7] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z};
-  const bool two = place & 8, one = place & 4;
-  uint32_t x[6], y[5];
+// the 16 bytes of shared memory that begin `place` (0 .. 15, a multiple of kSize) behind `at` (one of 16)
+template <int kSize> __device__ __forceinline__ uint4 zp_read_between(uint32_t at, int place) {
+  at += place & 8;
+  const uint2 a = zp_lds8(at), b = zp_lds8(at + 8), c = zp_lds8(at + 16);
+  const uint32_t w[6] = {a.x, a.y, b.x, b.y, c.x, c.y};
+  uint32_t y[5];
 #pragma unroll
-  for (int k = 0; k < 5; ++k) x[k] = two ? w[k + 2] : w[k];
-  x[5] = two ? b.w : w[5];
-#pragma unroll
-  for (int k = 0; k < 5; ++k) y[k] = one ? x[k + 1] : x[k];
+  for (int k = 0; k < 5; ++k) y[k] = place & 4 ? w[k + 1] : w[k];
   if constexpr (kSize == 2) {
     const int half = (place & 2) * 8;
 #pragma unroll
@@ -300,45 +322,56 @@ template <typename T> __device__ __forceinline__ void zp_cut(int q, int width, f
 }
 // Piece number i of a thread, of a row in a slot.  Elements past the row's end are zero.
 template <typename T, bool kAligned>
-__device__ __forceinline__ void zp_read(const ZpTeam &t, const char *slot, int place, int i, int width,
+__device__ __forceinline__ void zp_read(const ZpTeam &t, uint32_t slot, int place, int i, int width,
                                         float2 (&v)[kZpVec<T> / 2]) {
   const int q = t.lane + i * t.size;
   if constexpr (kAligned) {
-    zp_unpack<T>(*reinterpret_cast<const uint4 *>(slot + 16 * q), v);
+    zp_unpack<T>(zp_lds16(slot + 16 * q), v);
   } else {
-    zp_unpack<T>(zp_read_between<sizeof(T)>(slot, q, place), v);
+    zp_unpack<T>(zp_read_between<sizeof(T)>(slot + 16 * q, place), v);
     zp_cut<T>(q, width, v);
   }
 }
-// Results: aligned rows straight to memory; others into a slot, 16 bytes from its start, from where
-// zp_store_row takes them once the whole team has written.
+// Results: aligned rows straight to memory (`row`: the row's first element); others into a slot, 16 bytes
+// from its start, from where zp_store_row takes them once the whole team has written.
 template <typename T, bool kAligned>
-__device__ __forceinline__ void zp_write(const ZpTeam &t, char *row, char *slot, int i,
+__device__ __forceinline__ void zp_write(const ZpTeam &t, char *row, uint32_t slot, int i,
                                          const float2 (&v)[kZpVec<T> / 2]) {
   const int q = t.lane + i * t.size;
   if constexpr (kAligned) reinterpret_cast<uint4 *>(row)[q] = zp_pack<T>(v);
-  else reinterpret_cast<uint4 *>(slot)[q + 1] = zp_pack<T>(v);
+  else zp_sts16(slot + 16 * q + 16, zp_pack<T>(v));
 }
-template <typename T>
-__device__ __forceinline__ void zp_store_row(const ZpTeam &t, char *row, const char *slot, int width) {
-  const int place = (int)(reinterpret_cast<uintptr_t>(row) & 15), bytes = width * (int)sizeof(T);
-  char *const at = row - place;                // (a piece that begins before the row is not stored whole)
-  const int back = place ? 0 : 1;
-  for (int q = t.lane; 16 * q < place + bytes; q += t.size) {
-    const uint4 v = zp_read_between<sizeof(T)>(slot, q + back, (16 - place) & 15);
-    if (16 * q >= place && 16 * q + 16 <= place + bytes) {
-      *reinterpret_cast<uint4 *>(at + 16 * q) = v;
+template <typename T, int M>
+__device__ __forceinline__ void zp_store_row(const ZpTeam &t, char *row, uint32_t slot, int width) {
+  const int place = (int)(reinterpret_cast<uintptr_t>(row) & 15), end = place + width * (int)sizeof(T);
+  char *const to = row - place;                // (a piece that begins before the row is not stored whole)
+  const uint32_t from = place ? slot : slot + 16;
+  const int shift = (16 - place) & 15;
+#pragma unroll
+  for (int i = 0; i <= M; ++i) {
+    const int at = 16 * (t.lane + i * t.size);
+    if (at >= end) break;
+    const uint4 v = zp_read_between<sizeof(T)>(from + at, shift);
+    if (at >= place && at + 16 <= end) {
+      *reinterpret_cast<uint4 *>(to + at) = v;
     } else {
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      const int lo = place - at;
+      const unsigned n = (unsigned)((end < at + 16 ? end : at + 16) - (lo > 0 ? place : at));
+      const int begin = lo > 0 ? lo : 0;
 #pragma unroll
       for (int k = 0; k < kZpVec<T>; ++k) {
-        const int b = 16 * q + k * (int)sizeof(T);
-        if (b < place || b >= place + bytes) continue;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t *>(at + b) = w[k];
-        else *reinterpret_cast<uint16_t *>(at + b) = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
+        if ((unsigned)(k * (int)sizeof(T) - begin) >= n) continue;
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(to + at)[k] = w[k];
+        else reinterpret_cast<uint16_t *>(to + at)[k] = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
       }
     }
   }
+}
+
+// How many of the steps of `step` rows from row r on begin at a row that there is
+__device__ __forceinline__ int zp_steps(int64_t rows, int64_t r, int64_t step) {
+  return r < rows ? (int)((rows - r + step - 1) / step) : 0;
 }
 
 // ---- which of a thread's elements are kept ----------------------------------------------------------
@@ -390,18 +423,20 @@ __device__ __forceinline__ uint32_t zp_kept_bits(const ZpTeam &t, const ZpPhilox
 // ---- launches ---------------------------------------------------------------------------------------
 
 // How a call's rows are shared out: elements per thread and rows at a time, the team's size, whether pieces
-// of 16 bytes are aligned (of the rows, and of weight and bias), and the ring's sizes.
+// of 16 bytes are aligned (of the rows, and of weight and bias), whether every thread has all its pieces, and
+// the ring's sizes.
 struct ZpTeamPlan {
   int team, elements, rows;
-  bool aligned, vectors;
+  bool aligned, full, vectors;
   int slot, bytes, stages;                     // bytes of a slot, of the counters' bits of a team
   size_t smem;
   unsigned blocks;
 };
-// `arrays` come in per row; `last_per_element`: bytes of shared memory per element of a block's teams that
+// `arrays` come in per row; `results`: slots of a row that results pass through besides those of the ring;
+// `last_per_element`: bytes of shared memory per element of a block's teams that
 // the kernel needs when the ring is done with.  False: this does not fit.
-inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, size_t last_per_element, int elements,
-                         int rows, ZpTeamPlan &p) {
+inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, int results, size_t last_per_element,
+                         int elements, int rows, ZpTeamPlan &p) {
   const int64_t size = c.dtype == ZP_F32 ? 4 : 2;
   if (c.width > (int64_t)kZpTeamThreads * elements) return false;
   p.aligned = aligned;
@@ -411,15 +446,16 @@ inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, size_t l
   p.rows = rows;
   const int64_t need = zp_ceil_div(c.width, elements);
   for (p.team = 2; p.team < need; p.team *= 2) {}
+  p.full = aligned && (int64_t)p.team * elements == c.width;
   const int teams = kZpTeamThreads / p.team;
   p.slot = (int)(p.team * elements * size) + (aligned ? 0 : 48);
   p.bytes = aligned || !c.drop.state ? 0 : (int)zp_align_up((size_t)c.width / 8 + 3, 16);
-  const size_t red = sizeof(float) * 2 * 4 * kZpTeamWarps, fixed = red + (size_t)p.bytes * teams;
+  const size_t red = sizeof(float) * 2 * 4 * kZpTeamWarps, fixed = red + (size_t)(p.bytes + results * p.slot) * teams;
   const size_t last = last_per_element * kZpTeamThreads * elements, room = 226 * 1024;
   const size_t stage = (size_t)arrays * rows * p.slot * teams;
   p.stages = fixed + 4 * stage <= room ? 4 : fixed + 3 * stage <= room ? 3 : 2;
   if (fixed + p.stages * stage > room || fixed + last > room) return false;
-  p.smem = fixed + (p.stages * stage > last ? p.stages * stage : last);
+  p.smem = fixed + (p.stages * stage > last ? p.stages * stage : last);   // (results lie behind the ring)
   const int64_t units = zp_ceil_div(c.rows, rows * (p.team < 32 ? 32 / p.team : 1));
   p.blocks = (unsigned)(units < 148 ? units : 148);
   return true;

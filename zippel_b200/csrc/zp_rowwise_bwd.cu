@@ -8,42 +8,48 @@
 
 namespace {
 
-template <typename T, bool kAligned, int E, int R, bool kJoin>
+template <typename T, bool kAligned, bool kFull, int E, int R, bool kJoin>
 __global__ void __launch_bounds__(kZpTeamThreads, 1)
-norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
+norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant__ ZpTeamPlan p) {
   zp_after_previous();
   constexpr int V = kZpVec<T>, H = V / 2, M = E / V;
   constexpr bool kHeld = E <= 16;              // the weight, z and gy w stay in registers
   extern __shared__ __align__(16) char smem[];
   const ZpTeam t(p.team, reinterpret_cast<float *>(smem));
-  const int width = (int)c.width, teams = kZpTeamThreads / p.team, stages = p.stages;
+  const int width = (int)c.width, stages = p.stages;
   char *const after_red = smem + sizeof(float) * 2 * 4 * kZpTeamWarps;
   uint8_t *const bytes = reinterpret_cast<uint8_t *>(after_red) + t.index * p.bytes;
-  char *const rings = after_red + p.bytes * teams;
-  const int A = kJoin && c.dsum ? 3 : 2;
-  char *const ring = rings + (size_t)t.index * stages * A * R * p.slot;
+  char *const rings = after_red + p.bytes * (kZpTeamThreads / p.team);
+  const bool third = kJoin && c.dsum;          // of the arrays that come in
+  const uint32_t row_slots = (third ? 3 : 2) * p.slot, stage_bytes = R * row_slots, ring_bytes = stages * stage_bytes;
+  const uint32_t ring = zp_shared(rings) + t.index * ring_bytes;
+  const uint32_t results = zp_shared(rings) + (kZpTeamThreads / p.team) * ring_bytes +
+                           t.index * (c.dx && c.dres ? 2 : 1) * p.slot;              // behind the rings
+  // a walker takes R rows after one another of each of its teams
   const int64_t step = (int64_t)gridDim.x * t.walkers * t.per * R;
-  const int64_t first = ((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per * R + t.sub;
-  ZpSource sx(c.x, c.ldx, c.rows, c.width, sizeof(T), first, step, t.per);
-  ZpSource sy(c.dy, c.ldy, c.rows, c.width, sizeof(T), first, step, t.per);
-  ZpSource ss(c.dsum, c.lds, c.rows, c.width, sizeof(T), first, step, t.per);
-  int64_t coming = first;
-  auto fetch = [&](int stage) {
-    char *to = ring + stage * A * R * p.slot;
+  const int64_t first = (((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per + t.sub) * R;
+  ZpSource<kAligned> sx(t, c.x, c.ldx, c.rows, c.width, sizeof(T), first, step);
+  ZpSource<kAligned> sy(t, c.dy, c.ldy, c.rows, c.width, sizeof(T), first, step);
+  ZpSource<kAligned> ss(t, c.dsum, c.lds, c.rows, c.width, sizeof(T), first, step);
+  int n[R];                                    // turns in which this team has its row j
 #pragma unroll
-    for (int j = 0; j < R; ++j, to += A * p.slot) {
-      if (coming + j * t.per >= c.rows) continue;
-      zp_fetch_row<T, kAligned, M>(t, to, sx, sx.row + j * sx.next, width);
-      zp_fetch_row<T, kAligned, M>(t, to + p.slot, sy, sy.row + j * sy.next, width);
-      if (kJoin && A == 3) zp_fetch_row<T, kAligned, M>(t, to + 2 * p.slot, ss, ss.row + j * ss.next, width);
+  for (int j = 0; j < R; ++j) n[j] = zp_steps(c.rows, first + j, step);
+  const int turns = zp_steps(c.rows, first - t.sub * R, step);        // (a warp's teams go on together)
+  auto fetch = [&](int turn, uint32_t to) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if (turn >= n[j]) continue;
+      const uint32_t slot = to + j * row_slots;
+      zp_fetch_row<T, kAligned, kFull, M>(t, slot, sx, j, width);
+      zp_fetch_row<T, kAligned, kFull, M>(t, slot + p.slot, sy, j, width);
+      if (third) zp_fetch_row<T, kAligned, kFull, M>(t, slot + 2 * p.slot, ss, j, width);
     }
     sx.row += sx.step;
     sy.row += sy.step;
-    ss.row += ss.step;
-    coming += step;
+    if (kJoin) ss.row += ss.step;
     zp_copy_commit();
   };
-  for (int s = 0; s < stages - 1; ++s) fetch(s);
+  for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
 
   const bool wide = c.param_dtype == ZP_F32;
   auto column = [&](int i) { return (t.lane + i * t.size) * V; };
@@ -58,45 +64,45 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
   const float inv_w = 1.f / (float)width;
   const int64_t row_bytes = c.width * (int64_t)sizeof(T);
   float next_mean[R], next_rstd[R];
-  auto load_stats = [&](int64_t r0) {
+  const float *mean_at = c.mean_in + first, *rstd_at = c.rstd_in + first;
+  auto load_stats = [&](int turn) {
 #pragma unroll
     for (int j = 0; j < R; ++j)
-      if (r0 + j * t.per < c.rows) {
-        next_mean[j] = c.mean_in[r0 + j * t.per];
-        next_rstd[j] = c.rstd_in[r0 + j * t.per];
+      if (turn < n[j]) {
+        next_mean[j] = mean_at[j];
+        next_rstd[j] = rstd_at[j];
       }
+    mean_at += step;
+    rstd_at += step;
   };
 #pragma unroll
   for (int j = 0; j < R; ++j) next_mean[j] = next_rstd[j] = 0.f;
-  load_stats(first);
-  int stage = 0, turn = 0;
-  for (int64_t r0 = first; r0 - t.sub < c.rows; r0 += step) {
+  load_stats(0);
+  int64_t out = first * row_bytes;             // of the rows that are worked on, in every result
+  uint32_t slots = ring, behind = ring + (stages - 1) * stage_bytes;
+  for (int turn = 0; turn < turns; ++turn) {
     float mean[R], rstd[R], s[2 * R];
 #pragma unroll
     for (int j = 0; j < R; ++j) { mean[j] = next_mean[j]; rstd[j] = next_rstd[j]; }
     zp_copy_wait(stages);
-    if (!kAligned) t.sync();
-    fetch(stage == 0 ? stages - 1 : stage - 1);
-    load_stats(r0 + step);
-    char *const slots = ring + stage * A * R * p.slot;
-    stage = stage + 1 == stages ? 0 : stage + 1;
+    if (!kAligned) t.sync();                   // others' pieces are there; the last rows have been read
+    fetch(turn + stages - 1, behind);
+    load_stats(turn + 1);
     float2 z[kHeld ? R : 1][M][H], g[kHeld ? R : 1][M][H];
-    int mine[R];
     // z and gy w of row j, piece i, from the slots
     auto load = [&](int j, int i, float2 (&zz)[H], float2 (&gy)[H]) {
-      zp_read<T, kAligned>(t, slots + j * A * p.slot, sx.place_of(j), i, width, zz);
-      zp_read<T, kAligned>(t, slots + (j * A + 1) * p.slot, sy.place_of(j), i, width, gy);
+      zp_read<T, kAligned>(t, slots + j * row_slots, sx.place_of(j), i, width, zz);
+      zp_read<T, kAligned>(t, slots + j * row_slots + p.slot, sy.place_of(j), i, width, gy);
       const float2 minus = make_float2(-mean[j], -mean[j]), by = make_float2(rstd[j], rstd[j]);
 #pragma unroll
       for (int k = 0; k < H; ++k) zz[k] = __fmul2_rn(__fadd2_rn(zz[k], minus), by);
     };
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      mine[j] = r0 + j * t.per < c.rows ? width : 0;
       float2 s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (column(i) >= mine[j]) continue;
+        if (turn >= n[j] || (!kFull && column(i) >= width)) continue;
         float2 (&zz)[H] = z[kHeld ? j : 0][i], (&gz)[H] = g[kHeld ? j : 0][i];
         load(j, i, zz, gz);
         float2 ww[H];
@@ -113,20 +119,21 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
       s[2 * j] = s1.x + s1.y;
       s[2 * j + 1] = s2.x + s2.y;
     }
-    t.sum(s, turn++, !kAligned);
+    t.sum(s, turn, !kAligned);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const int64_t r = r0 + j * t.per;
       uint32_t kept = 0xffffffffu;
       if (kJoin && c.drop.state)
-        kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, mine[j] ? r : 0, width, bytes);
+        kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, turn < n[j] ? first + turn * step + j : 0, width, bytes);
       const float2 minus1 = make_float2(-s[2 * j] * inv_w, -s[2 * j] * inv_w);
       const float2 minus2 = make_float2(-s[2 * j + 1] * inv_w, -s[2 * j + 1] * inv_w);
       const float2 by = make_float2(rstd[j], rstd[j]);
-      char *const slot = slots + j * A * p.slot;
+      const uint32_t slot = slots + j * row_slots;
+      const int64_t at = out + j * row_bytes;
+      const uint32_t to = kHeld ? slot : results;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (column(i) >= mine[j]) continue;
+        if (turn >= n[j] || (!kFull && column(i) >= width)) continue;
         float2 o[H], q[H];
         if constexpr (kHeld) {
 #pragma unroll
@@ -141,38 +148,41 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
             o[k] = __fmul2_rn(__ffma2_rn(zz[k], minus2, __ffma2_rn(q[k], ww[k], minus1)), by);
         }
         if constexpr (!kJoin) {
-          if (c.dx) zp_write<T, kAligned>(t, static_cast<char *>(c.dx) + r * row_bytes, slot, i, o);
+          if (c.dx) zp_write<T, kAligned>(t, static_cast<char *>(c.dx) + at, to, i, o);
           continue;
         }
-        if (A == 3) {
+        if (third) {
           zp_read<T, kAligned>(t, slot + 2 * p.slot, ss.place_of(j), i, width, q);
 #pragma unroll
           for (int k = 0; k < H; ++k) o[k] = __fadd2_rn(o[k], q[k]);
         }
-        if (c.dres) zp_write<T, kAligned>(t, static_cast<char *>(c.dres) + r * row_bytes, slot, i, o);
+        if (c.dres) zp_write<T, kAligned>(t, static_cast<char *>(c.dres) + at, to, i, o);
         if (!c.dx) continue;
 #pragma unroll
         for (int k = 0; k < H; ++k) {
           const uint32_t two = kept >> (i * V + 2 * k);
           o[k] = make_float2(two & 1 ? o[k].x * c.drop.scale : 0.f, two & 2 ? o[k].y * c.drop.scale : 0.f);
         }
-        zp_write<T, kAligned>(t, static_cast<char *>(c.dx) + r * row_bytes, slot + p.slot, i, o);
+        zp_write<T, kAligned>(t, static_cast<char *>(c.dx) + at, c.dres ? to + p.slot : to, i, o);
       }
     }
     if constexpr (!kAligned) {
       t.sync();
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        const int64_t r = r0 + j * t.per;
-        if (!mine[j]) continue;
-        char *const slot = slots + j * A * p.slot;
-        if (kJoin && c.dres) zp_store_row<T>(t, static_cast<char *>(c.dres) + r * row_bytes, slot, width);
-        if (c.dx) zp_store_row<T>(t, static_cast<char *>(c.dx) + r * row_bytes, slot + (kJoin ? p.slot : 0), width);
+        if (turn >= n[j]) continue;
+        const int64_t at = out + j * row_bytes;
+        const uint32_t from = kHeld ? slots + j * row_slots : results;
+        if (kJoin && c.dres) zp_store_row<T, M>(t, static_cast<char *>(c.dres) + at, from, width);
+        if (c.dx) zp_store_row<T, M>(t, static_cast<char *>(c.dx) + at, kJoin && c.dres ? from + p.slot : from, width);
       }
+      sx.advance();
+      sy.advance();
+      ss.advance();
     }
-    sx.advance();
-    sy.advance();
-    ss.advance();
+    out += step * row_bytes;
+    behind = slots;
+    slots = slots + stage_bytes == ring + ring_bytes ? ring : slots + stage_bytes;
   }
   zp_copy_wait(2);
   if (!c.partial) return;
@@ -202,32 +212,36 @@ norm_bwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
       }
   }
   __syncthreads();
-  float *const out = c.partial + (size_t)blockIdx.x * 2 * c.width;
+  float *const part = c.partial + (size_t)blockIdx.x * 2 * c.width;
   for (int i = threadIdx.x; i < 2 * width; i += kZpTeamThreads) {
     const int at = i < width ? i : row + (i - width);
     float sum = 0.f;
     for (int k = 0; k < copies; ++k) sum += all[(size_t)k * 2 * row + at];
-    out[i] = sum;
+    part[i] = sum;
   }
 }
 
-template <typename T, bool kAligned, int E, int R, bool kJoin>
+bool is_join(const ZpNormCall &c) { return c.dsum || c.dres || c.drop.state; }
+
+template <typename T, bool kAligned, bool kFull, int E, int R, bool kJoin>
 int launch(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
   static ZpSmemOptIn opt_in;
-  if (int rc = zp_ensure_smem(norm_bwd_team_kernel<T, kAligned, E, R, kJoin>, p.smem, opt_in)) return rc;
-  zp_launch(norm_bwd_team_kernel<T, kAligned, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
+  if (int rc = zp_ensure_smem(norm_bwd_team_kernel<T, kAligned, kFull, E, R, kJoin>, p.smem, opt_in)) return rc;
+  zp_launch(norm_bwd_team_kernel<T, kAligned, kFull, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
   ZP_LAUNCH_CHECK("norm_bwd_team_kernel");
   return ZP_OK;
 }
-template <typename T, bool kAligned, bool kJoin>
+template <typename T, bool kAligned, bool kFull, bool kJoin>
 int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (p.elements == 8) return p.rows == 1 ? launch<T, kAligned, 8, 1, kJoin>(c, p, st) : launch<T, kAligned, 8, 2, kJoin>(c, p, st);
-  return p.elements == 16 ? launch<T, kAligned, 16, 1, kJoin>(c, p, st) : launch<T, kAligned, 32, 1, kJoin>(c, p, st);
+  if (p.elements == 8) return p.rows == 1 ? launch<T, kAligned, kFull, 8, 1, kJoin>(c, p, st) : launch<T, kAligned, kFull, 8, 2, kJoin>(c, p, st);
+  return p.elements == 16 ? launch<T, kAligned, kFull, 16, 1, kJoin>(c, p, st) : launch<T, kAligned, kFull, 32, 1, kJoin>(c, p, st);
+}
+template <typename T, bool kJoin> int by_alignment(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+  if (p.full) return by_elements<T, true, true, kJoin>(c, p, st);
+  return p.aligned ? by_elements<T, true, false, kJoin>(c, p, st) : by_elements<T, false, false, kJoin>(c, p, st);
 }
 template <typename T> int by_kind(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (c.dsum || c.dres || c.drop.state)
-    return p.aligned ? by_elements<T, true, true>(c, p, st) : by_elements<T, false, true>(c, p, st);
-  return p.aligned ? by_elements<T, true, false>(c, p, st) : by_elements<T, false, false>(c, p, st);
+  return is_join(c) ? by_alignment<T, true>(c, p, st) : by_alignment<T, false>(c, p, st);
 }
 
 }  // namespace
@@ -241,11 +255,16 @@ int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_
                        (!c.drop.state || c.width % 8 == 0);
   const int64_t n = c.rows * c.width, threads = (int64_t)148 * kZpTeamThreads;
   const int arrays = c.dsum ? 3 : 2;
+  const bool join = is_join(c);
   const size_t last = c.partial ? 2 * sizeof(float) : 0;
+  // (rows of many elements are read twice, so that their results cannot pass through the slots they came in)
+  const int results = aligned ? 0 : c.dx && c.dres ? 2 : 1;
   ZpTeamPlan p;
-  taken = c.dy && ((n >= threads * 32 && zp_team_plan(c, aligned, arrays, last, 8, 2, p)) ||
-                   zp_team_plan(c, aligned, arrays, last, 8, 1, p) || zp_team_plan(c, aligned, arrays, last, 16, 1, p) ||
-                   zp_team_plan(c, aligned, arrays, last, 32, 1, p));
+  taken = c.dy && ((join && n >= threads * 32 && zp_team_plan(c, aligned, arrays, 0, last, 8, 2, p)) ||
+                   (n >= threads * 32 && zp_team_plan(c, aligned, arrays, 0, last, 16, 1, p)) ||
+                   zp_team_plan(c, aligned, arrays, 0, last, 8, 1, p) ||
+                   zp_team_plan(c, aligned, arrays, 0, last, 16, 1, p) ||
+                   zp_team_plan(c, aligned, arrays, results, last, 32, 1, p));
   if (!taken) return ZP_OK;
   parts = (int)p.blocks;
   if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);

@@ -8,38 +8,40 @@
 namespace {
 
 // E elements of a thread in each of R rows at a time
-template <typename T, bool kAligned, int E, int R, bool kJoin>
+template <typename T, bool kAligned, bool kFull, int E, int R, bool kJoin>
 __global__ void __launch_bounds__(kZpTeamThreads, 1)
-norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
+norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant__ ZpTeamPlan p) {
   zp_after_previous();
   constexpr int V = kZpVec<T>, H = V / 2, M = E / V, A = kJoin ? 2 : 1;
   constexpr bool kHeld = E <= 16;              // weight and bias stay in registers
   extern __shared__ __align__(16) char smem[];
   const ZpTeam t(p.team, reinterpret_cast<float *>(smem));
-  const int width = (int)c.width, teams = kZpTeamThreads / p.team, stages = p.stages;
+  const int width = (int)c.width, stages = p.stages;
   char *const after_red = smem + sizeof(float) * 2 * 4 * kZpTeamWarps;
   uint8_t *const bytes = reinterpret_cast<uint8_t *>(after_red) + t.index * p.bytes;
-  char *const ring = after_red + p.bytes * teams + (size_t)t.index * stages * A * R * p.slot;
-  // a walker takes R rows of each of its teams, its teams' side by side; rows of a team are `per` apart
+  const uint32_t stage_bytes = A * R * p.slot, ring_bytes = stages * stage_bytes;
+  const uint32_t ring = zp_shared(after_red) + p.bytes * (kZpTeamThreads / p.team) + t.index * ring_bytes;
+  // a walker takes R rows after one another of each of its teams
   const int64_t step = (int64_t)gridDim.x * t.walkers * t.per * R;
-  const int64_t first = ((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per * R + t.sub;
-  ZpSource sx(c.x, c.ldx, c.rows, c.width, sizeof(T), first, step, t.per);
-  ZpSource sr(c.res, c.ldr, c.rows, c.width, sizeof(T), first, step, t.per);
-  int64_t coming = first;
-  auto fetch = [&](int stage) {
-    char *to = ring + stage * A * R * p.slot;
+  const int64_t first = (((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per + t.sub) * R;
+  ZpSource<kAligned> sx(t, c.x, c.ldx, c.rows, c.width, sizeof(T), first, step);
+  ZpSource<kAligned> sr(t, c.res, c.ldr, c.rows, c.width, sizeof(T), first, step);
+  int n[R];                                    // turns in which this team has its row j
 #pragma unroll
-    for (int j = 0; j < R; ++j, to += A * p.slot) {
-      if (coming + j * t.per >= c.rows) continue;
-      zp_fetch_row<T, kAligned, M>(t, to, sx, sx.row + j * sx.next, width);
-      if (kJoin) zp_fetch_row<T, kAligned, M>(t, to + p.slot, sr, sr.row + j * sr.next, width);
+  for (int j = 0; j < R; ++j) n[j] = zp_steps(c.rows, first + j, step);
+  const int turns = zp_steps(c.rows, first - t.sub * R, step);        // (a warp's teams go on together)
+  auto fetch = [&](int turn, uint32_t to) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if (turn >= n[j]) continue;
+      zp_fetch_row<T, kAligned, kFull, M>(t, to + j * A * p.slot, sx, j, width);
+      if (kJoin) zp_fetch_row<T, kAligned, kFull, M>(t, to + (j * A + 1) * p.slot, sr, j, width);
     }
     sx.row += sx.step;
-    sr.row += sr.step;
-    coming += step;
+    if (kJoin) sr.row += sr.step;
     zp_copy_commit();
   };
-  for (int s = 0; s < stages - 1; ++s) fetch(s);
+  for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
 
   const bool wide = c.param_dtype == ZP_F32;
   auto column = [&](int i) { return (t.lane + i * t.size) * V; };
@@ -52,30 +54,25 @@ norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
   const ZpPhiloxKey key = kJoin && c.drop.state ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
   const float inv_w = 1.f / (float)width;
   const int64_t row_bytes = c.width * (int64_t)sizeof(T);
-  int stage = 0;
-  for (int64_t r0 = first; r0 - t.sub < c.rows; r0 += step) {        // (a warp's teams go on together)
+  int64_t out = first * row_bytes;             // of the rows that are worked on, in every result
+  uint32_t slots = ring, behind = ring + (stages - 1) * stage_bytes;
+  for (int turn = 0; turn < turns; ++turn) {
     zp_copy_wait(stages);
     if (!kAligned) t.sync();                   // others' pieces are there; the last rows have been read
-    fetch(stage == 0 ? stages - 1 : stage - 1);
-    char *const slots = ring + stage * A * R * p.slot;
-    stage = stage + 1 == stages ? 0 : stage + 1;
+    fetch(turn + stages - 1, behind);
     float2 v[R][M][H];
     float s[R];
-    int mine[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const int64_t r = r0 + j * t.per;
-      mine[j] = r < c.rows ? width : 0;
-      char *const x = slots + j * A * p.slot, *const res = x + p.slot;
+      const bool mine = turn < n[j];
+      const uint32_t x = slots + j * A * p.slot, res = x + p.slot;
       uint32_t kept = 0xffffffffu;
       if (kJoin && c.drop.state)
-        kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, mine[j] ? r : 0, width, bytes);
+        kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, mine ? first + turn * step + j : 0, width, bytes);
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-#pragma unroll
-        for (int k = 0; k < H; ++k) v[j][i][k] = make_float2(0.f, 0.f);
-        if (column(i) >= mine[j]) continue;
+        if (!mine || (!kFull && column(i) >= width)) continue;
         zp_read<T, kAligned>(t, x, sx.place_of(j), i, width, v[j][i]);
         if constexpr (kJoin) {
           float2 q[H];
@@ -90,7 +87,7 @@ norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
           // rounded: what follows works on the sum as it is returned
           const uint4 packed = zp_pack<T>(v[j][i]);
           if (kAligned)
-            reinterpret_cast<uint4 *>(static_cast<char *>(c.sum) + r * row_bytes)[t.lane + i * t.size] = packed;
+            reinterpret_cast<uint4 *>(static_cast<char *>(c.sum) + out + j * row_bytes)[t.lane + i * t.size] = packed;
           zp_unpack<T>(packed, v[j][i]);
         }
 #pragma unroll
@@ -107,7 +104,7 @@ norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
       const float2 minus = make_float2(-s[j], -s[j]);
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (column(i) >= mine[j]) continue;
+        if (turn >= n[j] || (!kFull && column(i) >= width)) continue;
         if constexpr (kJoin && !kAligned)      // (the team has read all of this slot)
           zp_write<T, kAligned>(t, nullptr, slots + j * A * p.slot, i, v[j][i]);
 #pragma unroll
@@ -121,12 +118,12 @@ norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
     t.sum(q, 1, !kAligned);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const int64_t r = r0 + j * t.per;
       const float rstd = rsqrtf(q[j] * inv_w + c.eps);
       const float2 both = make_float2(rstd, rstd);
+      char *const y = static_cast<char *>(c.y) + out + j * row_bytes;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (column(i) >= mine[j]) continue;
+        if (turn >= n[j] || (!kFull && column(i) >= width)) continue;
         float2 ww[H], bb[H];
         if constexpr (!kHeld) {
           zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, ww);
@@ -136,44 +133,54 @@ norm_fwd_team_kernel(const ZpNormCall c, const ZpTeamPlan p) {
         for (int k = 0; k < H; ++k)
           v[j][i][k] = __ffma2_rn(__fmul2_rn(v[j][i][k], both), kHeld ? w[kHeld ? i : 0][k] : ww[k],
                                   kHeld ? b[kHeld ? i : 0][k] : bb[k]);
-        zp_write<T, kAligned>(t, static_cast<char *>(c.y) + r * row_bytes, slots + (j * A + A - 1) * p.slot, i, v[j][i]);
+        zp_write<T, kAligned>(t, y, slots + (j * A + A - 1) * p.slot, i, v[j][i]);
       }
-      if (c.mean && mine[j] && t.lane == 0) { c.mean[r] = s[j]; c.rstd[r] = rstd; }
+      if (t.lane == 0 && c.mean && turn < n[j]) {
+        const int64_t r = first + turn * step + j;
+        c.mean[r] = s[j];
+        c.rstd[r] = rstd;
+      }
     }
     if constexpr (!kAligned) {
       t.sync();
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        const int64_t r = r0 + j * t.per;
-        if (!mine[j]) continue;
-        zp_store_row<T>(t, static_cast<char *>(c.y) + r * row_bytes, slots + (j * A + A - 1) * p.slot, width);
-        if (kJoin) zp_store_row<T>(t, static_cast<char *>(c.sum) + r * row_bytes, slots + j * A * p.slot, width);
+        if (turn >= n[j]) continue;
+        const int64_t at = out + j * row_bytes;
+        zp_store_row<T, M>(t, static_cast<char *>(c.y) + at, slots + (j * A + A - 1) * p.slot, width);
+        if (kJoin) zp_store_row<T, M>(t, static_cast<char *>(c.sum) + at, slots + j * A * p.slot, width);
       }
+      sx.advance();
+      sr.advance();
     }
-    sx.advance();
-    sr.advance();
+    out += step * row_bytes;
+    behind = slots;
+    slots = slots + stage_bytes == ring + ring_bytes ? ring : slots + stage_bytes;
   }
   zp_copy_wait(2);
 }
 
-template <typename T, bool kAligned, int E, int R, bool kJoin>
+template <typename T, bool kAligned, bool kFull, int E, int R, bool kJoin>
 int launch(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
   static ZpSmemOptIn opt_in;
-  if (int rc = zp_ensure_smem(norm_fwd_team_kernel<T, kAligned, E, R, kJoin>, p.smem, opt_in)) return rc;
-  zp_launch(norm_fwd_team_kernel<T, kAligned, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
+  if (int rc = zp_ensure_smem(norm_fwd_team_kernel<T, kAligned, kFull, E, R, kJoin>, p.smem, opt_in)) return rc;
+  zp_launch(norm_fwd_team_kernel<T, kAligned, kFull, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
   ZP_LAUNCH_CHECK("norm_fwd_team_kernel");
   return ZP_OK;
 }
-template <typename T, bool kAligned, bool kJoin>
+template <typename T, bool kAligned, bool kFull, bool kJoin>
 int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (p.elements == 8) return p.rows == 1 ? launch<T, kAligned, 8, 1, kJoin>(c, p, st) : launch<T, kAligned, 8, 2, kJoin>(c, p, st);
-  if (p.elements == 16)
-    return p.rows == 1 ? launch<T, kAligned, 16, 1, kJoin>(c, p, st) : launch<T, kAligned, 16, 2, kJoin>(c, p, st);
-  return launch<T, kAligned, 32, 1, kJoin>(c, p, st);
+  if (p.elements == 8) return launch<T, kAligned, kFull, 8, 1, kJoin>(c, p, st);
+  if (p.elements == 32) return launch<T, kAligned, kFull, 32, 1, kJoin>(c, p, st);
+  return p.rows == 1 ? launch<T, kAligned, kFull, 16, 1, kJoin>(c, p, st)
+                     : launch<T, kAligned, kFull, 16, 2, kJoin>(c, p, st);
+}
+template <typename T, bool kJoin> int by_alignment(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+  if (p.full) return by_elements<T, true, true, kJoin>(c, p, st);
+  return p.aligned ? by_elements<T, true, false, kJoin>(c, p, st) : by_elements<T, false, false, kJoin>(c, p, st);
 }
 template <typename T> int by_kind(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (c.res) return p.aligned ? by_elements<T, true, true>(c, p, st) : by_elements<T, false, true>(c, p, st);
-  return p.aligned ? by_elements<T, true, false>(c, p, st) : by_elements<T, false, false>(c, p, st);
+  return c.res ? by_alignment<T, true>(c, p, st) : by_alignment<T, false>(c, p, st);
 }
 
 }  // namespace
@@ -185,15 +192,13 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
                        zp_piece_aligned(c.y, c.width, size) &&
                        (!c.res || (zp_piece_aligned(c.res, c.ldr, size) && zp_piece_aligned(c.sum, c.width, size))) &&
                        (!c.drop.state || c.width % 8 == 0);
-  // the more elements a thread has, the less the rest of a row's work weighs; few rows are spread over
-  // more threads instead
   const int64_t n = c.rows * c.width, threads = (int64_t)148 * kZpTeamThreads;
   const int arrays = c.res ? 2 : 1;
   ZpTeamPlan p;
-  taken = (n >= threads * 64 && zp_team_plan(c, aligned, arrays, 0, 16, 2, p)) ||
-          (n >= threads * 32 && zp_team_plan(c, aligned, arrays, 0, 8, 2, p)) ||
-          zp_team_plan(c, aligned, arrays, 0, 8, 1, p) || zp_team_plan(c, aligned, arrays, 0, 16, 1, p) ||
-          zp_team_plan(c, aligned, arrays, 0, 32, 1, p);
+  taken = (n >= threads * 64 && zp_team_plan(c, aligned, arrays, 0, 0, 16, 2, p)) ||
+          (n >= threads * 32 && zp_team_plan(c, aligned, arrays, 0, 0, 16, 1, p)) ||
+          zp_team_plan(c, aligned, arrays, 0, 0, 8, 1, p) || zp_team_plan(c, aligned, arrays, 0, 0, 16, 1, p) ||
+          zp_team_plan(c, aligned, arrays, 0, 0, 32, 1, p);
   if (!taken) return ZP_OK;
   if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);
   if (c.dtype == ZP_F16) return by_kind<__half>(c, p, st);
