@@ -11,6 +11,7 @@ import pathlib
 
 _LIB_PATH = pathlib.Path(__file__).resolve().parent / "libzippel_b200.so"
 _lib = None
+_torch = None
 
 
 class ZpError(RuntimeError):
@@ -166,13 +167,17 @@ def run(device, name: str, *args) -> None:
     """Library function ``name`` with the current stream of ``device`` as its last argument and
     ``device`` current.  Spares what the context manager and the stream object cost when the device
     is current already, a tenth of the host's share of a small call."""
-    import torch
-    fn = getattr(load(), name)
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)), name)
+    global _torch
+    if _torch is None:
+        import torch as _torch
+    fn, index = getattr(_lib or load(), name), device.index
+    if _torch._C._cuda_getDevice() == index:
+        status = fn(*args, _torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+        with _torch.cuda.device(device):
+            status = fn(*args, _torch.cuda.current_stream().cuda_stream)
+    if status:
+        raise ZpError(status, name)
 
 
 def check(status: int, where: str) -> None:

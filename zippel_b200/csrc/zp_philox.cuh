@@ -12,42 +12,60 @@
 
 #include <stdint.h>
 
+// The key of a call: the words of its ten rounds, worked out once, and the upper half of the counter.
 struct ZpPhiloxKey {
-  uint32_t k0, k1, c2, c3;
+  uint32_t k0[10], k1[10], c2, c3;
 };
 
 __device__ __forceinline__ ZpPhiloxKey zp_philox_key(const int64_t *__restrict__ state) {
   const uint64_t seed = (uint64_t)state[0], offset = (uint64_t)state[1];
-  return {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)};
+  ZpPhiloxKey key;
+  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    key.k0[i] = k0;
+    key.k1[i] = k1;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  key.c2 = (uint32_t)offset;
+  key.c3 = (uint32_t)(offset >> 32);
+  return key;
 }
 
 // the 128 bits of elements 8 * group .. 8 * group + 7
 __device__ __forceinline__ uint4 zp_philox(const ZpPhiloxKey &key, uint64_t group) {
   uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = key.c2, c3 = key.c3;
-  uint32_t k0 = key.k0, k1 = key.k1;
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ key.k0[i];
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ key.k1[i];
     c3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
 
-// bit j set: element 8 * group + j is kept (its 16 bits are at least `threshold`)
-__device__ __forceinline__ uint32_t zp_philox_kept(const ZpPhiloxKey &key, uint64_t group,
-                                                   uint32_t threshold) {
-  const uint4 w = zp_philox(key, group);
+// The two elements of a word, kept (times scale) or zero: 16 bits h are at least the threshold t exactly if
+// h 2^16 > limit = t 2^16 - 1, which for the upper half needs no shift.  1 <= t <= 2^16.
+__device__ __forceinline__ uint32_t zp_drop_limit(uint32_t threshold) { return (threshold << 16) - 1; }
+__device__ __forceinline__ float2 zp_drop_pair(float2 v, uint32_t word, uint32_t limit, float scale) {
+  const float2 by = __fmul2_rn(v, make_float2(scale, scale));
+  return make_float2((word << 16) > limit ? by.x : 0.f, word > limit ? by.y : 0.f);
+}
+
+// bit j set: element j of a counter's eight is kept
+__device__ __forceinline__ uint32_t zp_kept_of(const uint4 &w, uint32_t limit) {
   const uint32_t words[4] = {w.x, w.y, w.z, w.w};
   uint32_t kept = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    kept |= ((words[j] & 0xFFFFu) >= threshold ? 1u : 0u) << (2 * j);
-    kept |= ((words[j] >> 16) >= threshold ? 1u : 0u) << (2 * j + 1);
+    kept |= ((words[j] << 16) > limit ? 1u : 0u) << (2 * j);
+    kept |= (words[j] > limit ? 1u : 0u) << (2 * j + 1);
   }
   return kept;
+}
+__device__ __forceinline__ uint32_t zp_philox_kept(const ZpPhiloxKey &key, uint64_t group, uint32_t limit) {
+  return zp_kept_of(zp_philox(key, group), limit);
 }

@@ -29,99 +29,134 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
   return s;
 }
 
-// Dropout where groups of eight elements (one counter's) lie in aligned pieces of 16 bytes: `per_row`
-// groups a row, a warp 32 kAhead pieces at a time.  Bound by memory, with the generator close behind: of
-// some 75 integer instructions per group 20 are wide products.  In fp32 a piece is half a group: of two
-// neighbouring lanes each works out the counter of one of two pieces, and they swap.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-dropout_pieces_kernel(int64_t groups, uint32_t per_row, const T *__restrict__ x, int64_t ldx, ZpDrop drop,
-                      T *__restrict__ y, int64_t ldy) {
-  zp_after_previous();
-  constexpr int kAhead = 4, V = kZpVec<T>, kPieces = 8 / V;        // pieces of a group
-  const ZpPhiloxKey key = zp_philox_key(drop.state);
-  const int lane = threadIdx.x % 32;
-  const int64_t pieces = groups * kPieces, step = (int64_t)gridDim.x * kThreads * kAhead;
-  const bool flat = per_row == 0, small = groups <= 0xffffffffll;
-  for (int64_t p0 = (int64_t)(blockIdx.x * kThreads + threadIdx.x - lane) * kAhead; p0 < pieces; p0 += step) {
-    uint4 in[kAhead];
-    int64_t to[kAhead];
+// Dropout.  Each thread writes pieces of 16 bytes, kAhead of them 32 apart, whose loads are on the way together.
+// Bound by memory, with the generator close behind: of some 60 integer instructions for eight elements 20
+// are wide products.  In fp32 a piece is half of a counter's elements: of two neighbouring lanes each works
+// out the counter of one of two pieces, and they swap words.
+//   kFlat    one row of aligned pieces from end to end
+//   kRows    `per_row` aligned pieces a row
+//   kGather  y lies row behind row; a piece of x is put together from the two that it lies in, at the end of
+//            a row (or of x) from its elements
+enum { kFlat, kRows, kGather };
+// The words of kAhead pieces of a lane.
+template <typename T, int kAhead>
+__device__ __forceinline__ void kept_words(const ZpPhiloxKey &key, int64_t p0, int lane,
+                                           uint32_t (&w)[kAhead][kZpVec<T> / 2]) {
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int64_t p = p0 + 32 * i + lane;
-      if (p >= pieces) continue;
-      int64_t from = p * V;
-      to[i] = p * V;
-      if (!flat) {
-        const int64_t g = p / kPieces, r = small ? (uint32_t)g / per_row : g / per_row;
-        const int64_t c = (g - r * per_row) * 8 + p % kPieces * V;
-        from = r * ldx + c;
-        to[i] = r * ldy + c;
-      }
-      in[i] = __ldcs(reinterpret_cast<const uint4 *>(x + from));
+      const uint4 q = zp_philox(key, p0 + 32 * i + lane);
+      w[i][0] = q.x; w[i][1] = q.y; w[i][2] = q.z; w[i][3] = q.w;
     }
+  } else {
+    const bool odd = lane & 1;
 #pragma unroll
-    for (int i = 0; i < kAhead; i += kPieces) {
-      uint32_t kept[kPieces];
-      if constexpr (kPieces == 1) {
-        kept[0] = zp_philox_kept(key, p0 + 32 * i + lane, drop.threshold);
-      } else {
-        const int odd = lane & 1;
-        const uint32_t mine = zp_philox_kept(key, (p0 + 32 * (i + odd) + lane) / 2, drop.threshold);
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-        kept[0] = odd ? other >> 4 : mine;
-        kept[1] = odd ? mine >> 4 : other;
-      }
-#pragma unroll
-      for (int h = 0; h < kPieces; ++h) {
-        if (p0 + 32 * (i + h) + lane >= pieces) continue;
-        float2 v[V / 2];
-        zp_unpack<T>(in[i + h], v);
-#pragma unroll
-        for (int k = 0; k < V / 2; ++k)
-          v[k] = make_float2(kept[h] >> (2 * k) & 1 ? v[k].x * drop.scale : 0.f,
-                             kept[h] >> (2 * k + 1) & 1 ? v[k].y * drop.scale : 0.f);
-        __stcs(reinterpret_cast<uint4 *>(y + to[i + h]), zp_pack<T>(v));
-      }
+    for (int i = 0; i < kAhead; i += 2) {
+      const uint4 q = zp_philox(key, (p0 + 32 * (i + odd) + lane) / 2);
+      const uint32_t a = __shfl_xor_sync(0xffffffffu, odd ? q.x : q.z, 1);
+      const uint32_t b = __shfl_xor_sync(0xffffffffu, odd ? q.y : q.w, 1);
+      w[i][0] = odd ? a : q.x; w[i][1] = odd ? b : q.y;
+      w[i + 1][0] = odd ? q.z : a; w[i + 1][1] = odd ? q.w : b;
     }
   }
 }
 
-// Elements first .. rows * width - 1 wherever they lie: a warp goes through 256 of them, works out the 32
-// counters and hands each lane its bits; element by element the accesses are still side by side.
+template <typename T, int kHow>
+__global__ void __launch_bounds__(kThreads, 4)
+dropout_pieces_kernel(int64_t pieces, int64_t per_row, int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx,
+                      ZpDrop drop, T *__restrict__ y, int64_t ldy) {
+  zp_after_previous();
+  constexpr int kAhead = 4, V = kZpVec<T>;
+  const ZpPhiloxKey key = zp_philox_key(drop.state);
+  const uint32_t limit = zp_drop_limit(drop.threshold);
+  const int lane = threadIdx.x % 32;
+  const int64_t step = (int64_t)gridDim.x * kThreads * kAhead;
+  const bool small = rows * width <= 0xffffffffll;
+  for (int64_t p0 = (int64_t)(blockIdx.x * kThreads + threadIdx.x - lane) * kAhead; p0 < pieces; p0 += step) {
+    uint4 in[kAhead];
+    T *to[kHow == kRows ? kAhead : 1];
+    const int left = (int)(pieces - p0 < 32 * kAhead ? pieces - p0 : 32 * kAhead) - lane;       // of this lane's
+    if constexpr (kHow == kFlat) {
+      const uint4 *const from = reinterpret_cast<const uint4 *>(x) + p0 + lane;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (32 * i < left) in[i] = __ldcs(from + 32 * i);
+    } else if constexpr (kHow == kRows) {
+      int64_t q = p0 + lane, r = small ? (uint32_t)q / (uint32_t)per_row : q / per_row;        // row, piece of it
+      q -= r * per_row;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        to[i] = y + r * ldy + q * V;
+        if (32 * i < left) in[i] = __ldcs(reinterpret_cast<const uint4 *>(x + r * ldx + q * V));
+        q += 32;
+        if (q >= per_row) {
+          const int64_t more = per_row >= 32 ? 1 : q / per_row;
+          r += more;
+          q -= more * per_row;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int64_t e = (p0 + 32 * i + lane) * V;
+        if (32 * i >= left) continue;
+        const int64_t r = small ? (uint32_t)e / (uint32_t)width : e / width, c = e - r * width;
+        const char *const at = reinterpret_cast<const char *>(x + r * ldx + c);
+        const int place = (int)(reinterpret_cast<uintptr_t>(at) & 15);
+        const char *const from = at - place;
+        const char *const end = reinterpret_cast<const char *>(x + (rows - 1) * ldx + width);
+        if (c + V <= width && from >= reinterpret_cast<const char *>(x) && from + 32 <= end) {
+          const uint4 a = *reinterpret_cast<const uint4 *>(from), b = *reinterpret_cast<const uint4 *>(from + 16);
+          in[i] = zp_between<sizeof(T)>(a, b, place);
+        } else {
+          uint32_t w[4] = {0, 0, 0, 0};
+          int64_t rr = r, cc = c;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const T v = x[rr * ldx + cc];
+            if constexpr (sizeof(T) == 4) w[k] = *reinterpret_cast<const uint32_t *>(&v);
+            else w[k / 2] |= (uint32_t)*reinterpret_cast<const uint16_t *>(&v) << (16 * (k & 1));
+            if (++cc == width) { cc = 0; ++rr; }
+          }
+          in[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+    uint32_t words[kAhead][V / 2];
+    kept_words<T, kAhead>(key, p0, lane, words);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (32 * i >= left) continue;
+      float2 v[V / 2];
+      zp_unpack<T>(in[i], v);
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) v[k] = zp_drop_pair(v[k], words[i][k], limit, drop.scale);
+      uint4 *const out = reinterpret_cast<uint4 *>(kHow == kRows ? to[kHow == kRows ? i : 0] : y + (p0 + lane) * V);
+      __stcs(kHow == kRows ? out : out + 32 * i, zp_pack<T>(v));
+    }
+  }
+}
+
+// Elements first .. rows * width - 1 wherever they lie: the last ones of a call, and results that are not row
+// behind row.  A warp goes through 256 of them, works out the 32 counters and hands each lane its bits.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 dropout_elements_kernel(int64_t first, int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, ZpDrop drop,
                         T *__restrict__ y, int64_t ldy) {
   zp_after_previous();
   const ZpPhiloxKey key = zp_philox_key(drop.state);
+  const uint32_t limit = zp_drop_limit(drop.threshold);
   const int lane = threadIdx.x % 32;
   const int64_t n = rows * width, step = (int64_t)gridDim.x * kThreads * 8;
   for (int64_t e0 = first + (int64_t)(blockIdx.x * kThreads + threadIdx.x - lane) * 8; e0 < n; e0 += step) {
-    float v[8];
-    int64_t to[8];
-    int64_t r = 0, c = e0 + lane;
-    if (rows > 1) {
-      r = n <= 0xffffffffll ? (uint32_t)c / (uint32_t)width : c / width;
-      c -= r * width;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = 0.f;
-      to[j] = r * ldy + c;
-      if (e0 + 32 * j + lane < n) v[j] = zp_float(x[r * ldx + c]);
-      c += 32;
-      if (c >= width && rows > 1) {
-        const int64_t more = width > 32 ? 1 : c / width;
-        r += more;
-        c -= more * width;
-      }
-    }
-    const uint32_t mine = zp_philox_kept(key, e0 / 8 + lane, drop.threshold);
+    const uint32_t mine = zp_philox_kept(key, e0 / 8 + lane, limit);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t kept = __shfl_sync(0xffffffffu, mine, 4 * j + lane / 8) >> (lane % 8) & 1;
-      if (e0 + 32 * j + lane < n) y[to[j]] = zp_rounded<T>(kept ? v[j] * drop.scale : 0.f);
+      const int64_t e = e0 + 32 * j + lane;
+      if (e >= n) continue;
+      const int64_t r = e / width, c = e - r * width;
+      y[r * ldy + c] = zp_rounded<T>(kept ? zp_float(x[r * ldx + c]) * drop.scale : 0.f);
     }
   }
 }
@@ -146,7 +181,7 @@ norm_fwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ld
       const ZpPhiloxKey key = drop.state ? zp_philox_key(drop.state) : ZpPhiloxKey{};
       for (int64_t c = threadIdx.x; c < width; c += kThreads) {
         const uint64_t i = (uint64_t)(r * width + c);
-        const bool kept = !drop.state || (zp_philox_kept(key, i / 8, drop.threshold) >> (i % 8) & 1);
+        const bool kept = !drop.state || (zp_philox_kept(key, i / 8, zp_drop_limit(drop.threshold)) >> (i % 8) & 1);
         sum[r * width + c] = zp_rounded<T>(zp_float(res[r * ldr + c]) +
                                            (kept ? zp_float(in[c]) * drop.scale : 0.f));
       }
@@ -196,7 +231,7 @@ norm_bwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ld
       if (dres) dres[r * width + c] = zp_rounded<T>(g);
       if (dx) {
         const uint64_t i = (uint64_t)(r * width + c);
-        const bool kept = !drop.state || (zp_philox_kept(key, i / 8, drop.threshold) >> (i % 8) & 1);
+        const bool kept = !drop.state || (zp_philox_kept(key, i / 8, zp_drop_limit(drop.threshold)) >> (i % 8) & 1);
         dx[r * width + c] = zp_rounded<T>(kept ? g * drop.scale : 0.f);
       }
     }
@@ -274,23 +309,27 @@ unsigned blocks_for(int64_t n, int64_t most) { return (unsigned)std::max<int64_t
 
 template <typename T> int run_dropout(int64_t rows, int64_t width, const void *x, int64_t ldx, const ZpDrop &drop,
                                       void *y, int64_t ldy, cudaStream_t st) {
+  constexpr int V = kZpVec<T>;
   const T *in = static_cast<const T *>(x);
   T *out = static_cast<T *>(y);
-  if ((ldx == width && ldy == width) || rows == 1) {         // one row, and all of it that is whole groups
+  const bool behind = ldy == width || rows == 1;             // y lies row behind row
+  if (behind && (ldx == width || rows == 1)) {               // one row from end to end
     width *= rows;
     rows = 1;
     ldx = ldy = width;
   }
-  const bool pieces = !misplaced(x, 16) && !misplaced(y, 16) &&
-                      (rows == 1 || (width % 8 == 0 && width / 8 <= 0xffffffffll && ldx * sizeof(T) % 16 == 0 &&
-                                     ldy * sizeof(T) % 16 == 0));
-  int64_t first = 0;
-  if (pieces) {
-    const int64_t groups = rows * width / 8;
-    first = groups * 8;
-    if (groups > 0) {
-      zp_launch(dropout_pieces_kernel<T>, blocks_for(zp_ceil_div(groups * (8 / kZpVec<T>), 4 * kThreads), 148 * 8),
-                kThreads, 0, st, groups, rows == 1 ? 0u : (uint32_t)(width / 8), in, ldx, drop, out, ldy);
+  const bool whole = !misplaced(x, 16) && !misplaced(y, 16) &&
+                     (rows == 1 || (width % 8 == 0 && ldx % V == 0 && ldy % V == 0));
+  int64_t first = 0;                                          // elements that go by pieces, whole counters of them
+  if (whole || (behind && !misplaced(y, 16))) {
+    first = rows * width / 8 * 8;
+    const int64_t pieces = first / V;
+    const unsigned blocks = blocks_for(zp_ceil_div(pieces, 4 * kThreads), 148 * 8);
+    if (pieces > 0) {
+      const auto kernel = !whole      ? dropout_pieces_kernel<T, kGather>
+                          : rows == 1 ? dropout_pieces_kernel<T, kFlat>
+                                      : dropout_pieces_kernel<T, kRows>;
+      zp_launch(kernel, blocks, kThreads, 0, st, pieces, width / V, rows, width, in, ldx, drop, out, ldy);
       ZP_LAUNCH_CHECK("dropout_pieces_kernel");
     }
   }
@@ -395,8 +434,12 @@ int zp_dropout(int64_t rows, int64_t width, int dtype, const void *x, int64_t ld
   if (!make_drop(p, state, drop) || !state || misplaced(state, 8) || bad_rows(x, rows, width, ldx, dtype) ||
       bad_rows(y, rows, width, ldy, dtype))
     return ZP_ERR_INVALID_ARG;
-  drop.state = state;                          // (p = 0 copies)
   cudaStream_t st = (cudaStream_t)stream;
+  const size_t size = type_bytes(dtype);
+  if (!drop.state) {                           // nothing is dropped
+    ZP_CUDA(cudaMemcpy2DAsync(y, ldy * size, x, ldx * size, width * size, rows, cudaMemcpyDeviceToDevice, st));
+    return ZP_OK;
+  }
   if (dtype == ZP_F32) return run_dropout<float>(rows, width, x, ldx, drop, y, ldy, st);
   if (dtype == ZP_F16) return run_dropout<__half>(rows, width, x, ldx, drop, y, ldy, st);
   return run_dropout<__nv_bfloat16>(rows, width, x, ldx, drop, y, ldy, st);

@@ -22,7 +22,7 @@
 
 struct ZpDrop {                     // dropout of a call; state null: nothing is dropped
   const int64_t *state;
-  uint32_t threshold;
+  uint32_t threshold;               // of 65536
   float scale;
 };
 
@@ -294,11 +294,8 @@ __device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, uint32_t slot, con
   }
 }
 
-// the 16 bytes of shared memory that begin `place` (0 .. 15, a multiple of kSize) behind `at` (one of 16)
-template <int kSize> __device__ __forceinline__ uint4 zp_read_between(uint32_t at, int place) {
-  at += place & 8;
-  const uint2 a = zp_lds8(at), b = zp_lds8(at + 8), c = zp_lds8(at + 16);
-  const uint32_t w[6] = {a.x, a.y, b.x, b.y, c.x, c.y};
+// bytes place .. place + 15 (place 0 .. 15, a multiple of kSize) of two pieces of 16 side by side
+template <int kSize> __device__ __forceinline__ uint4 zp_shifted(const uint32_t (&w)[6], int place) {
   uint32_t y[5];
 #pragma unroll
   for (int k = 0; k < 5; ++k) y[k] = place & 4 ? w[k + 1] : w[k];
@@ -308,6 +305,19 @@ template <int kSize> __device__ __forceinline__ uint4 zp_read_between(uint32_t a
     for (int k = 0; k < 4; ++k) y[k] = __funnelshift_r(y[k], y[k + 1], half);
   }
   return make_uint4(y[0], y[1], y[2], y[3]);
+}
+template <int kSize> __device__ __forceinline__ uint4 zp_between(const uint4 &a, const uint4 &b, int place) {
+  const bool two = place & 8;
+  const uint32_t w[6] = {two ? a.z : a.x, two ? a.w : a.y, two ? b.x : a.z, two ? b.y : a.w, two ? b.z : b.x,
+                         two ? b.w : b.y};
+  return zp_shifted<kSize>(w, place);
+}
+// ... in shared memory, from `at` (a multiple of 16) on
+template <int kSize> __device__ __forceinline__ uint4 zp_read_between(uint32_t at, int place) {
+  at += place & 8;
+  const uint2 a = zp_lds8(at), b = zp_lds8(at + 8), c = zp_lds8(at + 16);
+  const uint32_t w[6] = {a.x, a.y, b.x, b.y, c.x, c.y};
+  return zp_shifted<kSize>(w, place);
 }
 
 // zeroes what of piece q lies past the row's end
@@ -375,50 +385,75 @@ __device__ __forceinline__ int zp_steps(int64_t rows, int64_t r, int64_t step) {
 }
 
 // ---- which of a thread's elements are kept ----------------------------------------------------------
-// Bit i * V + k of the result: element k of the thread's piece i of row r is kept.
-//   aligned, 16-bit   a piece is one counter's eight elements
+// For each pair of elements of each piece:
+//   aligned, 16-bit   a piece is one counter's eight elements, a pair one of its words
 //   aligned, fp32     a piece is half of them: of two neighbours each works out one of two counters, and
-//                     they swap
+//                     they swap words
 //   other rows        the team works out the row's counters, eight bits each into `bytes`
 //                     [width / 8 + 3], and every thread looks up its own
-// All threads of a warp come here together.
-template <typename T, bool kAligned, int E>
-__device__ __forceinline__ uint32_t zp_kept_bits(const ZpTeam &t, const ZpPhiloxKey &key, uint32_t threshold,
-                                                 int64_t r, int width, uint8_t *bytes) {
-  uint32_t bits = 0;
-  if constexpr (kAligned && sizeof(T) == 2) {
-    const uint64_t first = (uint64_t)r * (uint32_t)(width / 8) + t.lane;
+// kWords: kept as words, which saves two instructions an element; else as a bit per element, where registers
+// are short.
+template <typename T, bool kAligned, bool kWords, int E> struct ZpKept {
+  static_assert(kAligned || !kWords, "");
+  static constexpr int H = kZpVec<T> / 2;
+  uint32_t w[kWords ? E / 2 : 1];
+
+  // (all threads of a warp come here together)
+  __device__ __forceinline__ void find(const ZpTeam &t, const ZpPhiloxKey &key, uint32_t limit, int64_t r, int width,
+                                       uint8_t *bytes) {
+    if constexpr (kAligned) {
+      if (!kWords) w[0] = 0;
+      const uint64_t first = (uint64_t)r * (uint32_t)(width / 8);
+      const int odd = t.lane & 1;
 #pragma unroll
-    for (int i = 0; i < E / 8; ++i) bits |= zp_philox_kept(key, first + i * t.size, threshold) << (8 * i);
-  } else if constexpr (kAligned) {
-    const uint64_t first = (uint64_t)r * (uint32_t)(width / 8);
-    const int odd = t.lane & 1;
+      for (int i = 0; i < E / 8; ++i) {
+        // fp32: of pieces 2i and 2i + 1 the even lane works out the first one's counter, the odd one the other's
+        const int place = sizeof(T) == 2 ? t.lane + i * t.size : (t.lane + (2 * i + odd) * t.size) / 2;
+        uint4 q = zp_philox(key, first + place);
+        if constexpr (kWords) {
+          if constexpr (sizeof(T) == 4) {      // first half of a counter for the even lane
+            const uint32_t a = __shfl_xor_sync(0xffffffffu, odd ? q.x : q.z, 1);
+            const uint32_t b = __shfl_xor_sync(0xffffffffu, odd ? q.y : q.w, 1);
+            q = odd ? make_uint4(a, b, q.z, q.w) : make_uint4(q.x, q.y, a, b);
+          }
+          w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+        } else {
+          uint32_t mine = zp_kept_of(q, limit);
+          if constexpr (sizeof(T) == 4) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+            mine = odd ? other >> 4 | (mine & 0xf0) : (mine & 15) | (other & 15) << 4;
+          }
+          w[0] |= mine << (8 * i);
+        }
+      }
+    } else {
+      constexpr int V = kZpVec<T>;
+      const uint64_t e0 = (uint64_t)r * (uint64_t)width;
+      const int groups = (int)((e0 + width - 1) / 8 - e0 / 8) + 1, place = (int)(e0 & 7);
+      t.sync();                                // the last row's have been looked up
+      for (int g = t.lane; g < groups; g += t.size) bytes[g] = (uint8_t)zp_philox_kept(key, e0 / 8 + g, limit);
+      t.sync();
+      w[0] = 0;
 #pragma unroll
-    for (int i = 0; i < E / 8; ++i) {
-      const uint32_t mine = zp_philox_kept(key, first + (t.lane + (2 * i + odd) * t.size) / 2, threshold);
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-      // piece 2i: the even lane's counter, piece 2i + 1: the odd one's; low half for the even lane
-      const uint32_t lo = odd ? other >> 4 : mine & 15, hi = odd ? mine >> 4 : other & 15;
-      bits |= (lo | hi << 4) << (8 * i);
-    }
-  } else {
-    constexpr int V = kZpVec<T>;
-    const uint64_t e0 = (uint64_t)r * (uint64_t)width;
-    const int groups = (int)((e0 + width - 1) / 8 - e0 / 8) + 1, place = (int)(e0 & 7);
-    t.sync();                                  // the last row's have been looked up
-    for (int g = t.lane; g < groups; g += t.size) bytes[g] = (uint8_t)zp_philox_kept(key, e0 / 8 + g, threshold);
-    t.sync();
-#pragma unroll
-    for (int i = 0; i < E / V; ++i) {
-      const int c = (t.lane + i * t.size) * V, at = (place + c) >> 3;
-      if (c < width) {
-        const uint32_t two = bytes[at] | (uint32_t)bytes[at + 1] << 8;
-        bits |= (two >> ((place + c) & 7) & ((1u << V) - 1)) << (i * V);
+      for (int i = 0; i < E / V; ++i) {
+        const int c = (t.lane + i * t.size) * V, at = (place + c) >> 3;
+        if (c < width) {
+          const uint32_t two = bytes[at] | (uint32_t)bytes[at + 1] << 8;
+          w[0] |= (two >> ((place + c) & 7) & ((1u << V) - 1)) << (i * V);
+        }
       }
     }
   }
-  return bits;
-}
+  // pair k of piece i
+  __device__ __forceinline__ float2 drop(float2 v, int i, int k, uint32_t limit, float scale) const {
+    if constexpr (kWords) {
+      return zp_drop_pair(v, w[i * H + k], limit, scale);
+    } else {
+      const uint32_t two = w[0] >> (2 * (i * H + k));
+      return make_float2(two & 1 ? v.x * scale : 0.f, two & 2 ? v.y * scale : 0.f);
+    }
+  }
+};
 
 // ---- launches ---------------------------------------------------------------------------------------
 

@@ -60,7 +60,9 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
 #pragma unroll
     for (int k = 0; k < H; ++k) gw[i][k] = gb[i][k] = make_float2(0.f, 0.f);
   }
-  const ZpPhiloxKey key = kJoin && c.drop.state ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
+  const bool drops = kJoin && c.drop.state;
+  const ZpPhiloxKey key = drops ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
+  const uint32_t limit = zp_drop_limit(c.drop.threshold);
   const float inv_w = 1.f / (float)width;
   const int64_t row_bytes = c.width * (int64_t)sizeof(T);
   float next_mean[R], next_rstd[R];
@@ -122,9 +124,8 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     t.sum(s, turn, !kAligned);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      uint32_t kept = 0xffffffffu;
-      if (kJoin && c.drop.state)
-        kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, turn < n[j] ? first + turn * step + j : 0, width, bytes);
+      ZpKept<T, kAligned, false, E> kept;
+      if (drops) kept.find(t, key, limit, turn < n[j] ? first + turn * step + j : 0, width, bytes);
       const float2 minus1 = make_float2(-s[2 * j] * inv_w, -s[2 * j] * inv_w);
       const float2 minus2 = make_float2(-s[2 * j + 1] * inv_w, -s[2 * j + 1] * inv_w);
       const float2 by = make_float2(rstd[j], rstd[j]);
@@ -159,10 +160,7 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
         if (c.dres) zp_write<T, kAligned>(t, static_cast<char *>(c.dres) + at, to, i, o);
         if (!c.dx) continue;
 #pragma unroll
-        for (int k = 0; k < H; ++k) {
-          const uint32_t two = kept >> (i * V + 2 * k);
-          o[k] = make_float2(two & 1 ? o[k].x * c.drop.scale : 0.f, two & 2 ? o[k].y * c.drop.scale : 0.f);
-        }
+        for (int k = 0; k < H && drops; ++k) o[k] = kept.drop(o[k], i, k, limit, c.drop.scale);
         zp_write<T, kAligned>(t, static_cast<char *>(c.dx) + at, c.dres ? to + p.slot : to, i, o);
       }
     }
@@ -233,7 +231,9 @@ int launch(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
 }
 template <typename T, bool kAligned, bool kFull, bool kJoin>
 int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (p.elements == 8) return p.rows == 1 ? launch<T, kAligned, kFull, 8, 1, kJoin>(c, p, st) : launch<T, kAligned, kFull, 8, 2, kJoin>(c, p, st);
+  if constexpr (kAligned || !kJoin)
+    if (p.rows == 2) return launch<T, kAligned, kFull, 8, 2, kJoin>(c, p, st);
+  if (p.elements == 8) return launch<T, kAligned, kFull, 8, 1, kJoin>(c, p, st);
   return p.elements == 16 ? launch<T, kAligned, kFull, 16, 1, kJoin>(c, p, st) : launch<T, kAligned, kFull, 32, 1, kJoin>(c, p, st);
 }
 template <typename T, bool kJoin> int by_alignment(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
@@ -253,15 +253,18 @@ int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_
                        (!c.dx || zp_piece_aligned(c.dx, c.width, size)) &&
                        (!c.dres || zp_piece_aligned(c.dres, c.width, size)) &&
                        (!c.drop.state || c.width % 8 == 0);
-  const int64_t n = c.rows * c.width, threads = (int64_t)148 * kZpTeamThreads;
+  const int64_t each = c.rows * c.width / ((int64_t)148 * kZpTeamThreads);       // elements a thread
   const int arrays = c.dsum ? 3 : 2;
   const bool join = is_join(c);
   const size_t last = c.partial ? 2 * sizeof(float) : 0;
+  // Two rows at a time, as in the forward: 16384 x 4096 bf16 93 us -> 76, joined 153 -> 132, 400000 x 32 23 -> 20.
+  // Joined rows of a warp or less (60000 x 128 fp32 29 -> 31) or that are not aligned (30011 x 1001 fp16 150 -> 185:
+  // registers) are better one by one.
+  const bool two = each >= 32 && (!join || (aligned && c.width > 256));
   // (rows of many elements are read twice, so that their results cannot pass through the slots they came in)
   const int results = aligned ? 0 : c.dx && c.dres ? 2 : 1;
   ZpTeamPlan p;
-  taken = c.dy && ((join && n >= threads * 32 && zp_team_plan(c, aligned, arrays, 0, last, 8, 2, p)) ||
-                   (n >= threads * 32 && zp_team_plan(c, aligned, arrays, 0, last, 16, 1, p)) ||
+  taken = c.dy && ((two && zp_team_plan(c, aligned, arrays, 0, last, 8, 2, p)) ||
                    zp_team_plan(c, aligned, arrays, 0, last, 8, 1, p) ||
                    zp_team_plan(c, aligned, arrays, 0, last, 16, 1, p) ||
                    zp_team_plan(c, aligned, arrays, results, last, 32, 1, p));

@@ -51,7 +51,9 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, w[i]);
     zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, b[i]);
   }
-  const ZpPhiloxKey key = kJoin && c.drop.state ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
+  const bool drops = kJoin && c.drop.state;
+  const ZpPhiloxKey key = drops ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
+  const uint32_t limit = zp_drop_limit(c.drop.threshold);
   const float inv_w = 1.f / (float)width;
   const int64_t row_bytes = c.width * (int64_t)sizeof(T);
   int64_t out = first * row_bytes;             // of the rows that are worked on, in every result
@@ -66,9 +68,8 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     for (int j = 0; j < R; ++j) {
       const bool mine = turn < n[j];
       const uint32_t x = slots + j * A * p.slot, res = x + p.slot;
-      uint32_t kept = 0xffffffffu;
-      if (kJoin && c.drop.state)
-        kept = zp_kept_bits<T, kAligned, E>(t, key, c.drop.threshold, mine ? first + turn * step + j : 0, width, bytes);
+      ZpKept<T, kAligned, kAligned, E> kept;
+      if (drops) kept.find(t, key, limit, mine ? first + turn * step + j : 0, width, bytes);
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < M; ++i) {
@@ -79,9 +80,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
           zp_read<T, kAligned>(t, res, sr.place_of(j), i, width, q);
 #pragma unroll
           for (int k = 0; k < H; ++k) {
-            const uint32_t two = kept >> (i * V + 2 * k);
-            const float2 f = make_float2(two & 1 ? v[j][i][k].x * c.drop.scale : 0.f,
-                                         two & 2 ? v[j][i][k].y * c.drop.scale : 0.f);
+            const float2 f = drops ? kept.drop(v[j][i][k], i, k, limit, c.drop.scale) : v[j][i][k];
             v[j][i][k] = __fadd2_rn(q[k], f);
           }
           // rounded: what follows works on the sum as it is returned
@@ -172,8 +171,9 @@ template <typename T, bool kAligned, bool kFull, bool kJoin>
 int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
   if (p.elements == 8) return launch<T, kAligned, kFull, 8, 1, kJoin>(c, p, st);
   if (p.elements == 32) return launch<T, kAligned, kFull, 32, 1, kJoin>(c, p, st);
-  return p.rows == 1 ? launch<T, kAligned, kFull, 16, 1, kJoin>(c, p, st)
-                     : launch<T, kAligned, kFull, 16, 2, kJoin>(c, p, st);
+  if constexpr (sizeof(T) == 2)
+    if (p.rows == 2) return launch<T, kAligned, kFull, 16, 2, kJoin>(c, p, st);
+  return launch<T, kAligned, kFull, 16, 1, kJoin>(c, p, st);
 }
 template <typename T, bool kJoin> int by_alignment(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
   if (p.full) return by_elements<T, true, true, kJoin>(c, p, st);
@@ -192,11 +192,15 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
                        zp_piece_aligned(c.y, c.width, size) &&
                        (!c.res || (zp_piece_aligned(c.res, c.ldr, size) && zp_piece_aligned(c.sum, c.width, size))) &&
                        (!c.drop.state || c.width % 8 == 0);
-  const int64_t n = c.rows * c.width, threads = (int64_t)148 * kZpTeamThreads;
+  // Two rows at a time halve what joining the sums of a team of several warps costs (16384 x 4096 bf16 59 us ->
+  // 49), and leave the ring fewer stages (fp32 42 -> 50, joined without dropout 92 -> 99) and the blocks fewer
+  // turns to share out (60000 x 128 bf16 9.5 -> 10.4).  Few elements are spread over more threads.
+  const int64_t each = c.rows * c.width / ((int64_t)148 * kZpTeamThreads);       // elements a thread
   const int arrays = c.res ? 2 : 1;
+  const bool two = each >= 64 && c.width > 512 && size == 2 && (!c.res || c.drop.state);
   ZpTeamPlan p;
-  taken = (n >= threads * 64 && zp_team_plan(c, aligned, arrays, 0, 0, 16, 2, p)) ||
-          (n >= threads * 32 && zp_team_plan(c, aligned, arrays, 0, 0, 16, 1, p)) ||
+  taken = (two && zp_team_plan(c, aligned, arrays, 0, 0, 16, 2, p)) ||
+          (each >= 32 && zp_team_plan(c, aligned, arrays, 0, 0, 16, 1, p)) ||
           zp_team_plan(c, aligned, arrays, 0, 0, 8, 1, p) || zp_team_plan(c, aligned, arrays, 0, 0, 16, 1, p) ||
           zp_team_plan(c, aligned, arrays, 0, 0, 32, 1, p);
   if (!taken) return ZP_OK;
