@@ -3,7 +3,9 @@
     python -m zippel_b200.build [--force] [--verbose]
 
 Each ``csrc/*.cu`` is compiled to an object under ``csrc/_obj`` (skipped when newer than its
-sources) and the objects are linked into ``zippel_b200/libzippel_b200.so``.
+sources) and the objects are linked into ``zippel_b200/libzippel_b200.so``.  ``csrc/*_torch.cpp``, functions
+on torch tensors over that library, become extension modules beside it (``_rowwise``), for the torch and
+Python that build them.
 """
 
 from __future__ import annotations
@@ -20,6 +22,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = CSRC / "_obj"
 LIB = PKG / "libzippel_b200.so"
+ROWWISE = PKG / "_rowwise.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -72,7 +75,31 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode:
             raise RuntimeError("link failed:\n" + res.stdout + res.stderr)
+    build_rowwise(force)
     return LIB
+
+
+def build_rowwise(force: bool = False) -> pathlib.Path:
+    """The extension module of the operators over rows (``csrc/zp_rowwise_torch.cpp``)."""
+    src = CSRC / "zp_rowwise_torch.cpp"
+    if not force and not _stale(ROWWISE, [src, ROOT / "include" / "zippel_b200.h"]):
+        return ROWWISE
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    includes = [*cpp_extension.include_paths(), str(pathlib.Path(nvcc()).resolve().parent.parent / "include"),
+                sysconfig.get_paths()["include"], str(ROOT / "include")]
+    libs = pathlib.Path(torch.__file__).parent / "lib"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[a for i in includes for a in ("-isystem", i)], str(src), "-o", str(ROWWISE),
+           "-L", str(libs), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
+           "-L", str(PKG), "-lzippel_b200", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode:
+        raise RuntimeError("g++ failed on " + src.name + ":\n" + res.stdout + res.stderr)
+    return ROWWISE
 
 
 if __name__ == "__main__":
