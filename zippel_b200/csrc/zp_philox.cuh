@@ -12,21 +12,19 @@
 
 #include <stdint.h>
 
-// The key of a call: the words of its ten rounds, worked out once, and the upper half of the counter.
-struct ZpPhiloxKey {
-  uint32_t k0[10], k1[10], c2, c3;
+// The key of a call: the words of its ten rounds and the upper half of the counter.  kKept: all twenty words
+// worked out once, in registers; else from the first two each time, where registers are short.
+template <bool kKept> struct ZpPhiloxKey {
+  uint32_t k0[kKept ? 10 : 1], k1[kKept ? 10 : 1], c2, c3;
 };
 
-__device__ __forceinline__ ZpPhiloxKey zp_philox_key(const int64_t *__restrict__ state) {
+template <bool kKept> __device__ __forceinline__ ZpPhiloxKey<kKept> zp_philox_key(const int64_t *__restrict__ state) {
   const uint64_t seed = (uint64_t)state[0], offset = (uint64_t)state[1];
-  ZpPhiloxKey key;
-  uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+  ZpPhiloxKey<kKept> key;
 #pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    key.k0[i] = k0;
-    key.k1[i] = k1;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+  for (int i = 0; i < (kKept ? 10 : 1); ++i) {
+    key.k0[i] = (uint32_t)seed + i * 0x9E3779B9u;
+    key.k1[i] = (uint32_t)(seed >> 32) + i * 0xBB67AE85u;
   }
   key.c2 = (uint32_t)offset;
   key.c3 = (uint32_t)(offset >> 32);
@@ -34,14 +32,14 @@ __device__ __forceinline__ ZpPhiloxKey zp_philox_key(const int64_t *__restrict__
 }
 
 // the 128 bits of elements 8 * group .. 8 * group + 7
-__device__ __forceinline__ uint4 zp_philox(const ZpPhiloxKey &key, uint64_t group) {
+template <bool kKept> __device__ __forceinline__ uint4 zp_philox(const ZpPhiloxKey<kKept> &key, uint64_t group) {
   uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = key.c2, c3 = key.c3;
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ key.k0[i];
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ (kKept ? key.k0[kKept ? i : 0] : key.k0[0] + i * 0x9E3779B9u);
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ key.k1[i];
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ (kKept ? key.k1[kKept ? i : 0] : key.k1[0] + i * 0xBB67AE85u);
     c3 = (uint32_t)a;
   }
   return make_uint4(c0, c1, c2, c3);
@@ -66,6 +64,7 @@ __device__ __forceinline__ uint32_t zp_kept_of(const uint4 &w, uint32_t limit) {
   }
   return kept;
 }
-__device__ __forceinline__ uint32_t zp_philox_kept(const ZpPhiloxKey &key, uint64_t group, uint32_t limit) {
+template <bool kKept>
+__device__ __forceinline__ uint32_t zp_philox_kept(const ZpPhiloxKey<kKept> &key, uint64_t group, uint32_t limit) {
   return zp_kept_of(zp_philox(key, group), limit);
 }

@@ -40,7 +40,7 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 enum { kFlat, kRows, kGather };
 // The words of kAhead pieces of a lane.
 template <typename T, int kAhead>
-__device__ __forceinline__ void kept_words(const ZpPhiloxKey &key, int64_t p0, int lane,
+__device__ __forceinline__ void kept_words(const ZpPhiloxKey<true> &key, int64_t p0, int lane,
                                            uint32_t (&w)[kAhead][kZpVec<T> / 2]) {
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -67,7 +67,7 @@ dropout_pieces_kernel(int64_t pieces, int64_t per_row, int64_t rows, int64_t wid
                       ZpDrop drop, T *__restrict__ y, int64_t ldy) {
   zp_after_previous();
   constexpr int kAhead = 4, V = kZpVec<T>;
-  const ZpPhiloxKey key = zp_philox_key(drop.state);
+  const ZpPhiloxKey<true> key = zp_philox_key<true>(drop.state);
   const uint32_t limit = zp_drop_limit(drop.threshold);
   const int lane = threadIdx.x % 32;
   const int64_t step = (int64_t)gridDim.x * kThreads * kAhead;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads)
 dropout_elements_kernel(int64_t first, int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, ZpDrop drop,
                         T *__restrict__ y, int64_t ldy) {
   zp_after_previous();
-  const ZpPhiloxKey key = zp_philox_key(drop.state);
+  const ZpPhiloxKey<true> key = zp_philox_key<true>(drop.state);
   const uint32_t limit = zp_drop_limit(drop.threshold);
   const int lane = threadIdx.x % 32;
   const int64_t n = rows * width, step = (int64_t)gridDim.x * kThreads * 8;
@@ -178,7 +178,7 @@ norm_fwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ld
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *in = x + r * ldx;
     if (res) {
-      const ZpPhiloxKey key = drop.state ? zp_philox_key(drop.state) : ZpPhiloxKey{};
+      const ZpPhiloxKey<false> key = drop.state ? zp_philox_key<false>(drop.state) : ZpPhiloxKey<false>{};
       for (int64_t c = threadIdx.x; c < width; c += kThreads) {
         const uint64_t i = (uint64_t)(r * width + c);
         const bool kept = !drop.state || (zp_philox_kept(key, i / 8, zp_drop_limit(drop.threshold)) >> (i % 8) & 1);
@@ -220,7 +220,7 @@ norm_bwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ld
       s2 += gz * ((zp_float(x[r * ldx + c]) - mean) * rstd);
     }
     const float m1 = block_sum(s1, red) / (float)width, m2 = block_sum(s2, red) / (float)width;
-    const ZpPhiloxKey key = drop.state ? zp_philox_key(drop.state) : ZpPhiloxKey{};
+    const ZpPhiloxKey<false> key = drop.state ? zp_philox_key<false>(drop.state) : ZpPhiloxKey<false>{};
     for (int64_t c = threadIdx.x; c < width; c += kThreads) {
       float g = 0.f;
       if (dy) {

@@ -320,26 +320,22 @@ template <int kSize> __device__ __forceinline__ uint4 zp_read_between(uint32_t a
   return zp_shifted<kSize>(w, place);
 }
 
-// zeroes what of piece q lies past the row's end
-template <typename T> __device__ __forceinline__ void zp_cut(int q, int width, float2 (&v)[kZpVec<T> / 2]) {
-  const int left = width - q * kZpVec<T>;
-  if (left >= kZpVec<T>) return;
+// Piece number i of a thread, of a row in a slot.
+template <typename T, bool kAligned>
+__device__ __forceinline__ void zp_read(const ZpTeam &t, uint32_t slot, int place, int i, float2 (&v)[kZpVec<T> / 2]) {
+  const uint32_t at = slot + 16 * (t.lane + i * t.size);
+  zp_unpack<T>(kAligned ? zp_lds16(at) : zp_read_between<sizeof(T)>(at, place), v);
+}
+// How many elements of a piece that the row does not fill are the row's, in the thread that has it (else 0),
+// and zeroes in place of the others
+template <typename T> __device__ __forceinline__ int zp_tail(const ZpTeam &t, int width) {
+  return (width / kZpVec<T> & (t.size - 1)) == t.lane ? width % kZpVec<T> : 0;
+}
+template <typename T> __device__ __forceinline__ void zp_cut(int tail, float2 (&v)[kZpVec<T> / 2]) {
 #pragma unroll
   for (int k = 0; k < kZpVec<T> / 2; ++k) {
-    if (2 * k >= left) v[k].x = 0.f;
-    if (2 * k + 1 >= left) v[k].y = 0.f;
-  }
-}
-// Piece number i of a thread, of a row in a slot.  Elements past the row's end are zero.
-template <typename T, bool kAligned>
-__device__ __forceinline__ void zp_read(const ZpTeam &t, uint32_t slot, int place, int i, int width,
-                                        float2 (&v)[kZpVec<T> / 2]) {
-  const int q = t.lane + i * t.size;
-  if constexpr (kAligned) {
-    zp_unpack<T>(zp_lds16(slot + 16 * q), v);
-  } else {
-    zp_unpack<T>(zp_read_between<sizeof(T)>(slot + 16 * q, place), v);
-    zp_cut<T>(q, width, v);
+    if (2 * k >= tail) v[k].x = 0.f;
+    if (2 * k + 1 >= tail) v[k].y = 0.f;
   }
 }
 // Results: aligned rows straight to memory (`row`: the row's first element); others into a slot, 16 bytes
@@ -354,27 +350,31 @@ __device__ __forceinline__ void zp_write(const ZpTeam &t, char *row, uint32_t sl
 template <typename T, int M>
 __device__ __forceinline__ void zp_store_row(const ZpTeam &t, char *row, uint32_t slot, int width) {
   const int place = (int)(reinterpret_cast<uintptr_t>(row) & 15), end = place + width * (int)sizeof(T);
-  char *const to = row - place;                // (a piece that begins before the row is not stored whole)
+  char *const to = row - place;
   const uint32_t from = place ? slot : slot + 16;
   const int shift = (16 - place) & 15;
 #pragma unroll
   for (int i = 0; i <= M; ++i) {
     const int at = 16 * (t.lane + i * t.size);
-    if (at >= end) break;
-    const uint4 v = zp_read_between<sizeof(T)>(from + at, shift);
-    if (at >= place && at + 16 <= end) {
-      *reinterpret_cast<uint4 *>(to + at) = v;
+    if (i == M && 16 * M * t.size >= end) break;
+    if (at >= place && at + 16 <= end)
+      *reinterpret_cast<uint4 *>(to + at) = zp_read_between<sizeof(T)>(from + at, shift);
+  }
+  // what the row has of the pieces that it shares, element by element
+  constexpr int V = kZpVec<T>;
+  for (int k = t.lane; k < 2 * V; k += t.size) {
+    const int at = k < V ? k * (int)sizeof(T) : (end & ~15) + (k - V) * (int)sizeof(T);
+    const bool mine = k < V ? place && at >= place && at < end : (end & 15) && at >= (place ? 16 : 0) && at < end;
+    if (!mine) continue;
+    const uint32_t at_slot = slot + 16 + at - place;
+    if constexpr (sizeof(T) == 4) {
+      uint32_t v;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at_slot));
+      *reinterpret_cast<uint32_t *>(to + at) = v;
     } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      const int lo = place - at;
-      const unsigned n = (unsigned)((end < at + 16 ? end : at + 16) - (lo > 0 ? place : at));
-      const int begin = lo > 0 ? lo : 0;
-#pragma unroll
-      for (int k = 0; k < kZpVec<T>; ++k) {
-        if ((unsigned)(k * (int)sizeof(T) - begin) >= n) continue;
-        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(to + at)[k] = w[k];
-        else reinterpret_cast<uint16_t *>(to + at)[k] = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
-      }
+      uint16_t v;
+      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at_slot));
+      *reinterpret_cast<uint16_t *>(to + at) = v;
     }
   }
 }
@@ -399,7 +399,7 @@ template <typename T, bool kAligned, bool kWords, int E> struct ZpKept {
   uint32_t w[kWords ? E / 2 : 1];
 
   // (all threads of a warp come here together)
-  __device__ __forceinline__ void find(const ZpTeam &t, const ZpPhiloxKey &key, uint32_t limit, int64_t r, int width,
+  __device__ __forceinline__ void find(const ZpTeam &t, const ZpPhiloxKey<false> &key, uint32_t limit, int64_t r, int width,
                                        uint8_t *bytes) {
     if constexpr (kAligned) {
       if (!kWords) w[0] = 0;

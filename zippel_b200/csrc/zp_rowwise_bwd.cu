@@ -51,6 +51,7 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   };
   for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
 
+  const int tail = kAligned ? 0 : zp_tail<T>(t, width);
   const bool wide = c.param_dtype == ZP_F32;
   auto column = [&](int i) { return (t.lane + i * t.size) * V; };
   float2 w[kHeld ? M : 1][H], gw[M][H], gb[M][H];
@@ -61,7 +62,7 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     for (int k = 0; k < H; ++k) gw[i][k] = gb[i][k] = make_float2(0.f, 0.f);
   }
   const bool drops = kJoin && c.drop.state;
-  const ZpPhiloxKey key = drops ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
+  const ZpPhiloxKey<false> key = drops ? zp_philox_key<false>(c.drop.state) : ZpPhiloxKey<false>{};
   const uint32_t limit = zp_drop_limit(c.drop.threshold);
   const float inv_w = 1.f / (float)width;
   const int64_t row_bytes = c.width * (int64_t)sizeof(T);
@@ -93,8 +94,12 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     float2 z[kHeld ? R : 1][M][H], g[kHeld ? R : 1][M][H];
     // z and gy w of row j, piece i, from the slots
     auto load = [&](int j, int i, float2 (&zz)[H], float2 (&gy)[H]) {
-      zp_read<T, kAligned>(t, slots + j * row_slots, sx.place_of(j), i, width, zz);
-      zp_read<T, kAligned>(t, slots + j * row_slots + p.slot, sy.place_of(j), i, width, gy);
+      zp_read<T, kAligned>(t, slots + j * row_slots, sx.place_of(j), i, zz);
+      zp_read<T, kAligned>(t, slots + j * row_slots + p.slot, sy.place_of(j), i, gy);
+      if (!kAligned && tail && column(i) + tail == width) {
+        zp_cut<T>(tail, zz);
+        zp_cut<T>(tail, gy);
+      }
       const float2 minus = make_float2(-mean[j], -mean[j]), by = make_float2(rstd[j], rstd[j]);
 #pragma unroll
       for (int k = 0; k < H; ++k) zz[k] = __fmul2_rn(__fadd2_rn(zz[k], minus), by);
@@ -153,7 +158,7 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
           continue;
         }
         if (third) {
-          zp_read<T, kAligned>(t, slot + 2 * p.slot, ss.place_of(j), i, width, q);
+          zp_read<T, kAligned>(t, slot + 2 * p.slot, ss.place_of(j), i, q);
 #pragma unroll
           for (int k = 0; k < H; ++k) o[k] = __fadd2_rn(o[k], q[k]);
         }

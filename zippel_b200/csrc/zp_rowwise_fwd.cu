@@ -43,6 +43,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   };
   for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
 
+  const int tail = kAligned ? 0 : zp_tail<T>(t, width);
   const bool wide = c.param_dtype == ZP_F32;
   auto column = [&](int i) { return (t.lane + i * t.size) * V; };
   float2 w[kHeld ? M : 1][H], b[kHeld ? M : 1][H];
@@ -52,7 +53,13 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, b[i]);
   }
   const bool drops = kJoin && c.drop.state;
-  const ZpPhiloxKey key = drops ? zp_philox_key(c.drop.state) : ZpPhiloxKey{};
+  auto cut = [&](float2 (&v)[M][H]) {
+    if (kAligned || tail == 0) return;
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      if (column(i) + tail == width) zp_cut<T>(tail, v[i]);
+  };
+  const ZpPhiloxKey<false> key = drops ? zp_philox_key<false>(c.drop.state) : ZpPhiloxKey<false>{};
   const uint32_t limit = zp_drop_limit(c.drop.threshold);
   const float inv_w = 1.f / (float)width;
   const int64_t row_bytes = c.width * (int64_t)sizeof(T);
@@ -74,10 +81,10 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
 #pragma unroll
       for (int i = 0; i < M; ++i) {
         if (!mine || (!kFull && column(i) >= width)) continue;
-        zp_read<T, kAligned>(t, x, sx.place_of(j), i, width, v[j][i]);
+        zp_read<T, kAligned>(t, x, sx.place_of(j), i, v[j][i]);
         if constexpr (kJoin) {
           float2 q[H];
-          zp_read<T, kAligned>(t, res, sr.place_of(j), i, width, q);
+          zp_read<T, kAligned>(t, res, sr.place_of(j), i, q);
 #pragma unroll
           for (int k = 0; k < H; ++k) {
             const float2 f = drops ? kept.drop(v[j][i][k], i, k, limit, c.drop.scale) : v[j][i][k];
@@ -89,9 +96,14 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
             reinterpret_cast<uint4 *>(static_cast<char *>(c.sum) + out + j * row_bytes)[t.lane + i * t.size] = packed;
           zp_unpack<T>(packed, v[j][i]);
         }
-#pragma unroll
-        for (int k = 0; k < H; ++k) sum = __fadd2_rn(sum, v[j][i][k]);
       }
+      cut(v[j]);
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+        if (mine && (kFull || column(i) < width)) {
+#pragma unroll
+          for (int k = 0; k < H; ++k) sum = __fadd2_rn(sum, v[j][i][k]);
+        }
       s[j] = sum.x + sum.y;
     }
     t.sum(s, 0, !kAligned);
@@ -108,10 +120,14 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
           zp_write<T, kAligned>(t, nullptr, slots + j * A * p.slot, i, v[j][i]);
 #pragma unroll
         for (int k = 0; k < H; ++k) v[j][i][k] = __fadd2_rn(v[j][i][k], minus);
-        if constexpr (!kAligned) zp_cut<T>(t.lane + i * t.size, width, v[j][i]);
-#pragma unroll
-        for (int k = 0; k < H; ++k) sq = __ffma2_rn(v[j][i][k], v[j][i][k], sq);
       }
+      cut(v[j]);
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+        if (turn < n[j] && (kFull || column(i) < width)) {
+#pragma unroll
+          for (int k = 0; k < H; ++k) sq = __ffma2_rn(v[j][i][k], v[j][i][k], sq);
+        }
       q[j] = sq.x + sq.y;
     }
     t.sum(q, 1, !kAligned);
