@@ -194,6 +194,57 @@ def test_rows_that_lie_elsewhere(width, kind, dtype):
     near(b2[0], want.y, want.ty)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("width", [12, 100, 1002, 5001, 8186, 8190, 9999, 16377])
+def test_rows_that_share_pieces_of_memory(width, dtype):
+    """Widths that eight does not divide, of every class modulo eight, row behind row and from an odd address, few
+    rows (fewer than a cycle of eight) and more than there are blocks: gradients of the join with dropout."""
+    for rows in (1, 5, 400) if width < 2000 else (3, 310):
+        x, w, b, gy, gs = norm_case(rows, width, dtype, dtype, rows + width)
+        state, p = torch.tensor([rows, width]), 0.3
+        f = torch.ones(rows, width, dtype=torch.float64)
+        f = rowwise().dropout(f.float().cuda(), p, state.cuda()).double().cpu()        # (tested by itself)
+        xc, wc, bc, gc, sc = up(x, w, b, gy, gs)
+        for lie in (lambda t: t, lambda t: strided(t, "offset")):
+            leaves = [t.detach().requires_grad_() for t in (lie(xc), lie(sc), wc, bc)]
+            y, s = rowwise().dropout_add_layer_norm(*leaves, p, state.cuda(), EPS)
+            total = x.double() * f + gs.double()
+            near(s, total, rounding(dtype, total) + 4 * u * ((x.double() * f).abs() + total.abs()))
+            want = Want(s.detach().cpu(), w, b, gy, dtype, dtype, gs)
+            near(y, want.y, want.ty)
+            gx, gr, gw, gb = torch.autograd.grad([y, s], leaves, [lie(gc), lie(sc)])
+            near(gr, want.gx, want.tgx)
+            near(gx, want.gx * f, (want.line + 4 * u * want.gx.abs()) * f + rounding(dtype, want.gx * f))
+            near(gw, want.gw, want.tgw)
+            near(gb, want.gb, want.tgb)
+            plain = Want(x, w, b, gy, dtype, dtype)
+            leaves = [t.detach().requires_grad_() for t in (lie(xc), wc, bc)]
+            y = rowwise().layer_norm(*leaves, EPS)
+            near(y, plain.y, plain.ty)
+            for got, ref, tol in zip(torch.autograd.grad(y, leaves, lie(gc)), (plain.gx, plain.gw, plain.gb),
+                                     (plain.tgx, plain.tgw, plain.tgb)):
+                near(got, ref, tol)
+
+
+def test_neighbours_of_a_result_stay_as_they_are():
+    """Results of odd rows in the middle of an array, through the C ABI: what lies before and behind is not
+    touched, nor what the rows do not cover."""
+    from zippel_b200 import _lib
+    for rows, width, code, dt in ((9, 33, 0, F32), (9, 1001, 1, F16), (3, 7, 2, BF16), (300, 9, 1, F16)):
+        for lead in (0, 8, 16, 3):
+            x = torch.randn(rows, width, device="cuda").to(dt)
+            n = rows * width
+            y, s, stats = (torch.full((n + 64,), -7.0, device="cuda", dtype=dt) for _ in range(3))
+            stats = torch.empty(2, rows, device="cuda")
+            size = dt.itemsize
+            _lib.run(x.device, "zp_add_layernorm_forward", rows, width, code, x.data_ptr(), width, x.data_ptr(), width, 0.0,
+                     None, code, None, None, 1e-5, s.data_ptr() + lead * size, y.data_ptr() + lead * size,
+                     stats.data_ptr(), stats.data_ptr() + 4 * rows)
+            for t, ref in ((s, x + x), (y, torch.nn.functional.layer_norm((x + x).double(), (width,)).to(dt))):
+                assert bool((t[:lead] == -7).all()) and bool((t[lead + n:] == -7).all())
+                assert (t[lead:lead + n].view(rows, width).double() - ref.double()).abs().max() < 0.02
+
+
 def test_leading_axes():
     x, w, b, gy, _ = norm_case(4 * 6, 40, F32, F32, 1)
     want = Want(x, w, b, gy, F32, F32)

@@ -446,7 +446,7 @@ int zp_dropout(int64_t rows, int64_t width, int dtype, const void *x, int64_t ld
 }
 
 size_t zp_rowwise_work_bytes(int64_t rows, int64_t width) {
-  return rows > 0 && width > 0 ? sizeof(float) * 2 * (size_t)std::min<int64_t>(rows, ZP_ROWWISE_PARTS) * (size_t)width : 0;
+  return rows > 0 && width > 0 ? sizeof(float) * 2 * (size_t)std::min<int64_t>(rows + 7, ZP_ROWWISE_PARTS) * (size_t)width : 0;
 }
 
 int zp_layernorm_forward(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx, int param_dtype,

@@ -9,9 +9,16 @@
 // Rows come in through a ring in shared memory that asynchronous copies keep filled: the 6.5 TB/s of the
 // memory want some 40 KB in flight on every SM, which registers do not hold beside the sums.
 //   aligned rows   a thread copies the pieces that it works on itself: nobody waits for anybody
-//   other rows     the 16-byte pieces that the row lies in come as they are; after a barrier a thread puts
-//                  its pieces together from two of them, and results go the same way back
+//   cycled rows    of a width that eight does not divide, in arrays from end to end: row r begins r * width
+//                  mod 8 elements behind a border of eight, the same for every eighth row at least.  A team
+//                  takes rows of one such class alone, and its pieces are those of memory, the first and the last
+//                  shared with the neighbours: everything else is as with aligned rows
+//   shifted rows   all others.  The 16-byte pieces that the row lies in come as they are; after a barrier a
+//                  thread puts its pieces together from two of them, and results go the same way back
 #pragma once
+
+#include <initializer_list>
+#include <utility>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,7 +48,7 @@ struct ZpNormCall {
 
 // The kernels of teams (zp_rowwise_fwd.cu, zp_rowwise_bwd.cu); `taken` false: the call is not for them
 // and nothing was launched.  The backward leaves `parts` rows of partial sums {gw, gb} in c.partial, at
-// most ZP_ROWWISE_PARTS.
+// most ZP_ROWWISE_PARTS and seven more than there are rows.
 #define ZP_ROWWISE_PARTS 148
 int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st);
 int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_t st);
@@ -100,7 +107,7 @@ __device__ __forceinline__ float zp_param(const void *w, bool wide, int64_t c, f
   return wide ? static_cast<const float *>(w)[c] : zp_float(static_cast<const T *>(w)[c]);
 }
 
-// elements c .. c + V - 1 of one; vectors: they lie in aligned pieces of 16 bytes
+// elements c .. c + V - 1 of one (`otherwise` where there is none); vectors: they lie in aligned pieces of 16 bytes
 template <typename T>
 __device__ __forceinline__ void zp_params(const void *w, bool wide, bool vectors, int c, int width, float otherwise,
                                           float2 (&v)[kZpVec<T> / 2]) {
@@ -120,8 +127,8 @@ __device__ __forceinline__ void zp_params(const void *w, bool wide, bool vectors
   } else {
 #pragma unroll
     for (int k = 0; k < V / 2; ++k)
-      v[k] = make_float2(c + 2 * k < width ? zp_param<T>(w, wide, c + 2 * k, 0.f) : otherwise,
-                         c + 2 * k + 1 < width ? zp_param<T>(w, wide, c + 2 * k + 1, 0.f) : otherwise);
+      v[k] = make_float2((unsigned)(c + 2 * k) < (unsigned)width ? zp_param<T>(w, wide, c + 2 * k, 0.f) : otherwise,
+                         (unsigned)(c + 2 * k + 1) < (unsigned)width ? zp_param<T>(w, wide, c + 2 * k + 1, 0.f) : otherwise);
   }
 }
 
@@ -238,41 +245,78 @@ __device__ __forceinline__ void zp_sts16(uint32_t at, const uint4 &v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// One of the arrays that a ring brings in: the first of the next rows to fetch (and, in aligned arrays, this
-// thread's first piece of it), and the addresses that may be read.
-template <bool kAligned> struct ZpSource {
-  const char *row, *begin, *end;
-  int64_t step, next;                          // bytes from a team's rows to its next ones, and from row to row
-  int place;                                   // within 16 bytes, of the first of the rows that are worked on
-  __device__ __forceinline__ ZpSource(const ZpTeam &t, const void *base, int64_t ld, int64_t rows, int64_t width,
-                                      int size, int64_t first, int64_t rows_per_step) {
-    begin = static_cast<const char *>(base);
-    end = begin + ((rows - 1) * ld + width) * size;
-    row = begin + first * ld * size + (kAligned ? 16 * t.lane : 0);
-    step = rows_per_step * ld * size;
-    next = ld * size;
-    place = kAligned ? 0 : (int)(reinterpret_cast<uintptr_t>(row) & 15);
+enum ZpLying { kZpShifted, kZpAligned, kZpCycled };
+
+// A team's rows in a call: the first, how far from its rows of one turn to the next, from row to row within a
+// turn (kZpCycled: the cycle), in how many turns it has its row j and how many turns its warp makes; and how many
+// elements of its first piece lie before the row.
+template <int kLying, int R> struct ZpTeamRows {
+  int64_t first, step;
+  int next, turns, before;
+  int n[R];
+  __device__ __forceinline__ ZpTeamRows(const ZpTeam &t, int64_t rows, int width, int cycle_) {
+    const int cycle = kLying == kZpCycled ? cycle_ : 1;
+    const int64_t teams = (int64_t)gridDim.x * t.walkers * t.per;             // a multiple of the cycle
+    const int64_t team = ((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per;
+    auto first_of = [&](int64_t u) { return kLying == kZpCycled ? u % cycle + u / cycle * cycle * R : u * R; };
+    first = first_of(team + t.sub);
+    step = teams * R;
+    next = cycle;
+#pragma unroll
+    for (int j = 0; j < R; ++j) n[j] = steps(rows, first + j * next);
+    turns = steps(rows, first_of(team));                                      // (a warp's teams go on together)
+    before = kLying == kZpCycled ? (int)(first * width & 7) : 0;
   }
-  __device__ __forceinline__ int place_of(int j) const {
-    return kAligned ? 0 : (place + j * (int)(next & 15)) & 15;
-  }
-  __device__ __forceinline__ void advance() {
-    if (!kAligned) place = (place + (int)(step & 15)) & 15;
+  __device__ __forceinline__ int steps(int64_t rows, int64_t r) const {
+    return r < rows ? (int)((rows - r + step - 1) / step) : 0;
   }
 };
 
-// Row j of the next rows, `width` elements of T, into a slot.  kAligned: element c goes to byte
-// c * sizeof(T), each thread copies its own pieces (kFull: it has them all).  Else the row keeps its place
+// One of the arrays that a ring brings in: the first of the next rows to fetch (and, but for shifted rows, this
+// thread's first piece of it), and the addresses that may be read.
+template <int kLying> struct ZpSource {
+  static constexpr bool kShifted = kLying == kZpShifted;
+  const char *row, *begin, *end;
+  int64_t step, next;                          // bytes from a team's rows to its next ones, and from row to row
+  int place;                                   // within 16 bytes, of the first of the rows that are worked on
+  template <int R>
+  __device__ __forceinline__ ZpSource(const ZpTeam &t, const void *base, int64_t ld, int64_t rows, int64_t width,
+                                      int size, const ZpTeamRows<kLying, R> &own) {
+    begin = static_cast<const char *>(base);
+    end = begin + ((rows - 1) * ld + width) * size;
+    row = begin + (own.first * ld - own.before) * size + (kShifted ? 0 : 16 * t.lane);
+    step = own.step * ld * size;
+    next = own.next * ld * size;
+    place = kShifted ? (int)(reinterpret_cast<uintptr_t>(row) & 15) : 0;
+  }
+  __device__ __forceinline__ int place_of(int j) const { return kShifted ? (place + j * (int)(next & 15)) & 15 : 0; }
+  __device__ __forceinline__ void advance() {
+    if (kShifted) place = (place + (int)(step & 15)) & 15;
+  }
+};
+
+// Row j of the next rows, `width` elements of T, into a slot.  Each thread copies its own pieces (kFull: it has
+// them all), so that the row begins `before` elements behind the slot's begin; shifted rows keep their place
 // within 16 bytes.
-template <typename T, bool kAligned, bool kFull, int M>
-__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, uint32_t slot, const ZpSource<kAligned> &s, int j,
-                                             int width) {
+template <typename T, int kLying, bool kFull, int M>
+__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, uint32_t slot, const ZpSource<kLying> &s, int j,
+                                             int width, int before) {
+  constexpr int V = kZpVec<T>;
   const char *const row = j ? s.row + j * s.next : s.row;
-  if constexpr (kAligned) {
+  if constexpr (kLying != kZpShifted) {
     const uint32_t to = slot + 16 * t.lane;
 #pragma unroll
-    for (int i = 0; i < M; ++i)
-      if (kFull || (t.lane + i * t.size) * kZpVec<T> < width) zp_copy16(to + 16 * i * t.size, row + 16 * i * t.size);
+    for (int i = 0; i < M; ++i) {
+      const int c = (t.lane + i * t.size) * V - before;
+      if (kFull || (c < width && (kLying == kZpAligned || c + V > 0))) {
+        const char *const from = row + 16 * i * t.size;
+        if (kLying == kZpAligned || from + 16 <= s.end)
+          zp_copy16(to + 16 * i * t.size, from);
+        else                                   // the array's last piece: nothing is read behind its end
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 16 * i * t.size), "l"(from),
+                       "r"((int)(s.end - from)) : "memory");
+      }
+    }
   } else {
     const int place = (int)(reinterpret_cast<uintptr_t>(row) & 15), span = place + width * (int)sizeof(T);
     const char *const from = row - place;
@@ -321,31 +365,41 @@ template <int kSize> __device__ __forceinline__ uint4 zp_read_between(uint32_t a
 }
 
 // Piece number i of a thread, of a row in a slot.
-template <typename T, bool kAligned>
+template <typename T, int kLying>
 __device__ __forceinline__ void zp_read(const ZpTeam &t, uint32_t slot, int place, int i, float2 (&v)[kZpVec<T> / 2]) {
   const uint32_t at = slot + 16 * (t.lane + i * t.size);
-  zp_unpack<T>(kAligned ? zp_lds16(at) : zp_read_between<sizeof(T)>(at, place), v);
+  zp_unpack<T>(kLying == kZpShifted ? zp_read_between<sizeof(T)>(at, place) : zp_lds16(at), v);
 }
-// How many elements of a piece that the row does not fill are the row's, in the thread that has it (else 0),
-// and zeroes in place of the others
-template <typename T> __device__ __forceinline__ int zp_tail(const ZpTeam &t, int width) {
-  return (width / kZpVec<T> & (t.size - 1)) == t.lane ? width % kZpVec<T> : 0;
-}
-template <typename T> __device__ __forceinline__ void zp_cut(int tail, float2 (&v)[kZpVec<T> / 2]) {
+// zeroes in place of what of a piece from column c on lies outside the row
+template <typename T> __device__ __forceinline__ void zp_cut(int c, int width, float2 (&v)[kZpVec<T> / 2]) {
 #pragma unroll
   for (int k = 0; k < kZpVec<T> / 2; ++k) {
-    if (2 * k >= tail) v[k].x = 0.f;
-    if (2 * k + 1 >= tail) v[k].y = 0.f;
+    if ((unsigned)(c + 2 * k) >= (unsigned)width) v[k].x = 0.f;
+    if ((unsigned)(c + 2 * k + 1) >= (unsigned)width) v[k].y = 0.f;
   }
 }
-// Results: aligned rows straight to memory (`row`: the row's first element); others into a slot, 16 bytes
-// from its start, from where zp_store_row takes them once the whole team has written.
-template <typename T, bool kAligned>
-__device__ __forceinline__ void zp_write(const ZpTeam &t, char *row, uint32_t slot, int i,
+// Results, piece i from column c on.  `row`: where the team's first piece of the row goes; of a piece that the
+// row shares (`edge`: the thread may have one) its own elements alone are written.  Shifted rows go into a slot, 16
+// bytes from its start, from where zp_store_row takes them once the whole team has written.
+template <typename T, int kLying>
+__device__ __forceinline__ void zp_write(const ZpTeam &t, char *row, uint32_t slot, int i, int c, int width, bool edge,
                                          const float2 (&v)[kZpVec<T> / 2]) {
   const int q = t.lane + i * t.size;
-  if constexpr (kAligned) reinterpret_cast<uint4 *>(row)[q] = zp_pack<T>(v);
-  else zp_sts16(slot + 16 * q + 16, zp_pack<T>(v));
+  const uint4 packed = zp_pack<T>(v);
+  if constexpr (kLying == kZpShifted) {
+    zp_sts16(slot + 16 * q + 16, packed);
+  } else if (kLying == kZpAligned || !edge || (c >= 0 && c + kZpVec<T> <= width)) {
+    reinterpret_cast<uint4 *>(row)[q] = packed;
+  } else {
+    const uint32_t w[4] = {packed.x, packed.y, packed.z, packed.w};
+    T *const to = reinterpret_cast<T *>(row) + (size_t)q * kZpVec<T>;
+#pragma unroll
+    for (int k = 0; k < kZpVec<T>; ++k) {
+      if ((unsigned)(c + k) >= (unsigned)width) continue;
+      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t *>(to)[k] = w[k];
+      else reinterpret_cast<uint16_t *>(to)[k] = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
+    }
+  }
 }
 template <typename T, int M>
 __device__ __forceinline__ void zp_store_row(const ZpTeam &t, char *row, uint32_t slot, int width) {
@@ -379,31 +433,26 @@ __device__ __forceinline__ void zp_store_row(const ZpTeam &t, char *row, uint32_
   }
 }
 
-// How many of the steps of `step` rows from row r on begin at a row that there is
-__device__ __forceinline__ int zp_steps(int64_t rows, int64_t r, int64_t step) {
-  return r < rows ? (int)((rows - r + step - 1) / step) : 0;
-}
-
 // ---- which of a thread's elements are kept ----------------------------------------------------------
 // For each pair of elements of each piece:
-//   aligned, 16-bit   a piece is one counter's eight elements, a pair one of its words
-//   aligned, fp32     a piece is half of them: of two neighbours each works out one of two counters, and
+//   16-bit            a piece is one counter's eight elements, a pair one of its words
+//   fp32              a piece is half of them: of two neighbours each works out one of two counters, and
 //                     they swap words
-//   other rows        the team works out the row's counters, eight bits each into `bytes`
+//   shifted rows      the team works out the row's counters, eight bits each into `bytes`
 //                     [width / 8 + 3], and every thread looks up its own
 // kWords: kept as words, which saves two instructions an element; else as a bit per element, where registers
 // are short.
-template <typename T, bool kAligned, bool kWords, int E> struct ZpKept {
-  static_assert(kAligned || !kWords, "");
+template <typename T, int kLying, bool kWords, int E> struct ZpKept {
+  static_assert(kLying != kZpShifted || !kWords, "");
   static constexpr int H = kZpVec<T> / 2;
   uint32_t w[kWords ? E / 2 : 1];
 
   // (all threads of a warp come here together)
   __device__ __forceinline__ void find(const ZpTeam &t, const ZpPhiloxKey<false> &key, uint32_t limit, int64_t r, int width,
                                        uint8_t *bytes) {
-    if constexpr (kAligned) {
+    if constexpr (kLying != kZpShifted) {
       if (!kWords) w[0] = 0;
-      const uint64_t first = (uint64_t)r * (uint32_t)(width / 8);
+      const uint64_t first = (uint64_t)r * (uint32_t)width / 8;               // counter of the first piece
       const int odd = t.lane & 1;
 #pragma unroll
       for (int i = 0; i < E / 8; ++i) {
@@ -457,12 +506,12 @@ template <typename T, bool kAligned, bool kWords, int E> struct ZpKept {
 
 // ---- launches ---------------------------------------------------------------------------------------
 
-// How a call's rows are shared out: elements per thread and rows at a time, the team's size, whether pieces
-// of 16 bytes are aligned (of the rows, and of weight and bias), whether every thread has all its pieces, and
-// the ring's sizes.
+// How a call's rows are shared out: elements per thread and rows at a time, the team's size, how the rows
+// lie, whether every thread has all its pieces, whether weight and bias lie in aligned ones, and the ring's sizes.
 struct ZpTeamPlan {
   int team, elements, rows;
-  bool aligned, full, vectors;
+  int lying, cycle;                            // rows of a class are `cycle` apart
+  bool full, vectors;
   int slot, bytes, stages;                     // bytes of a slot, of the counters' bits of a team
   size_t smem;
   unsigned blocks;
@@ -470,21 +519,23 @@ struct ZpTeamPlan {
 // `arrays` come in per row; `results`: slots of a row that results pass through besides those of the ring;
 // `last_per_element`: bytes of shared memory per element of a block's teams that
 // the kernel needs when the ring is done with.  False: this does not fit.
-inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, int results, size_t last_per_element,
+inline bool zp_team_plan(const ZpNormCall &c, int lying, int arrays, int results, size_t last_per_element,
                          int elements, int rows, ZpTeamPlan &p) {
   const int64_t size = c.dtype == ZP_F32 ? 4 : 2;
-  if (c.width > (int64_t)kZpTeamThreads * elements) return false;
-  p.aligned = aligned;
-  p.vectors = c.width % (16 / size) == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0 &&
+  const int64_t span = lying == kZpCycled ? c.width + 7 : c.width;             // elements of a row's pieces
+  if (span > (int64_t)kZpTeamThreads * elements) return false;
+  p.lying = lying;
+  p.cycle = lying != kZpCycled ? 1 : c.width % 2 ? 8 : c.width % 4 ? 4 : 2;
+  p.vectors = lying != kZpCycled && c.width % (16 / size) == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0 &&
               reinterpret_cast<uintptr_t>(c.b) % 16 == 0;
   p.elements = elements;
   p.rows = rows;
-  const int64_t need = zp_ceil_div(c.width, elements);
+  const int64_t need = zp_ceil_div(span, elements);
   for (p.team = 2; p.team < need; p.team *= 2) {}
-  p.full = aligned && (int64_t)p.team * elements == c.width;
+  p.full = lying == kZpAligned && (int64_t)p.team * elements == c.width;
   const int teams = kZpTeamThreads / p.team;
-  p.slot = (int)(p.team * elements * size) + (aligned ? 0 : 48);
-  p.bytes = aligned || !c.drop.state ? 0 : (int)zp_align_up((size_t)c.width / 8 + 3, 16);
+  p.slot = (int)(p.team * elements * size) + (lying == kZpShifted ? 48 : 0);
+  p.bytes = lying != kZpShifted || !c.drop.state ? 0 : (int)zp_align_up((size_t)c.width / 8 + 3, 16);
   const size_t red = sizeof(float) * 2 * 4 * kZpTeamWarps, fixed = red + (size_t)(p.bytes + results * p.slot) * teams;
   const size_t last = last_per_element * kZpTeamThreads * elements, room = 226 * 1024;
   const size_t stage = (size_t)arrays * rows * p.slot * teams;
@@ -492,9 +543,21 @@ inline bool zp_team_plan(const ZpNormCall &c, bool aligned, int arrays, int resu
   if (fixed + p.stages * stage > room || fixed + last > room) return false;
   p.smem = fixed + (p.stages * stage > last ? p.stages * stage : last);   // (results lie behind the ring)
   const int64_t units = zp_ceil_div(c.rows, rows * (p.team < 32 ? 32 / p.team : 1));
-  p.blocks = (unsigned)(units < 148 ? units : 148);
+  // (classes of a cycle have as many teams each)
+  const int64_t by = p.cycle > teams ? p.cycle / teams : 1;
+  p.blocks = (unsigned)(units < 148 / by * by ? zp_ceil_div(units, by) * by : 148 / by * by);
   return true;
 }
-inline bool zp_piece_aligned(const void *p, int64_t ld, size_t size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ((size_t)ld * size) % 16 == 0;
+// How the rows of an array of a call lie; the call's are shifted where one array's are
+inline int zp_lying(const ZpNormCall &c, const void *p, int64_t ld) {
+  const int64_t size = c.dtype == ZP_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(p) % 16) return kZpShifted;
+  if (c.width * size % 16 == 0 && ld * size % 16 == 0 && (!c.drop.state || c.width % 8 == 0)) return kZpAligned;
+  return ld == c.width && c.width % 8 ? kZpCycled : kZpShifted;
+}
+inline int zp_lying(const ZpNormCall &c, std::initializer_list<std::pair<const void *, int64_t>> arrays) {
+  int found = -1;                              // (one width makes no array aligned and another cycled)
+  for (const auto &a : arrays)
+    if (a.first && found != kZpShifted) found = zp_lying(c, a.first, a.second);
+  return found;
 }

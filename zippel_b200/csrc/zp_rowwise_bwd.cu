@@ -8,7 +8,7 @@
 
 namespace {
 
-template <typename T, bool kAligned, bool kFull, int E, int R, bool kJoin>
+template <typename T, int kLying, bool kFull, int E, int R, bool kJoin>
 __global__ void __launch_bounds__(kZpTeamThreads, 1)
 norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant__ ZpTeamPlan p) {
   zp_after_previous();
@@ -25,24 +25,18 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   const uint32_t ring = zp_shared(rings) + t.index * ring_bytes;
   const uint32_t results = zp_shared(rings) + (kZpTeamThreads / p.team) * ring_bytes +
                            t.index * (c.dx && c.dres ? 2 : 1) * p.slot;              // behind the rings
-  // a walker takes R rows after one another of each of its teams
-  const int64_t step = (int64_t)gridDim.x * t.walkers * t.per * R;
-  const int64_t first = (((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per + t.sub) * R;
-  ZpSource<kAligned> sx(t, c.x, c.ldx, c.rows, c.width, sizeof(T), first, step);
-  ZpSource<kAligned> sy(t, c.dy, c.ldy, c.rows, c.width, sizeof(T), first, step);
-  ZpSource<kAligned> ss(t, c.dsum, c.lds, c.rows, c.width, sizeof(T), first, step);
-  int n[R];                                    // turns in which this team has its row j
-#pragma unroll
-  for (int j = 0; j < R; ++j) n[j] = zp_steps(c.rows, first + j, step);
-  const int turns = zp_steps(c.rows, first - t.sub * R, step);        // (a warp's teams go on together)
+  const ZpTeamRows<kLying, R> own(t, c.rows, width, p.cycle);
+  ZpSource<kLying> sx(t, c.x, c.ldx, c.rows, c.width, sizeof(T), own);
+  ZpSource<kLying> sy(t, c.dy, c.ldy, c.rows, c.width, sizeof(T), own);
+  ZpSource<kLying> ss(t, c.dsum, c.lds, c.rows, c.width, sizeof(T), own);
   auto fetch = [&](int turn, uint32_t to) {
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      if (turn >= n[j]) continue;
+      if (turn >= own.n[j]) continue;
       const uint32_t slot = to + j * row_slots;
-      zp_fetch_row<T, kAligned, kFull, M>(t, slot, sx, j, width);
-      zp_fetch_row<T, kAligned, kFull, M>(t, slot + p.slot, sy, j, width);
-      if (third) zp_fetch_row<T, kAligned, kFull, M>(t, slot + 2 * p.slot, ss, j, width);
+      zp_fetch_row<T, kLying, kFull, M>(t, slot, sx, j, width, own.before);
+      zp_fetch_row<T, kLying, kFull, M>(t, slot + p.slot, sy, j, width, own.before);
+      if (third) zp_fetch_row<T, kLying, kFull, M>(t, slot + 2 * p.slot, ss, j, width, own.before);
     }
     sx.row += sx.step;
     sy.row += sy.step;
@@ -51,9 +45,13 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   };
   for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
 
-  const int tail = kAligned ? 0 : zp_tail<T>(t, width);
   const bool wide = c.param_dtype == ZP_F32;
-  auto column = [&](int i) { return (t.lane + i * t.size) * V; };
+  auto column = [&](int i) { return (t.lane + i * t.size) * V - own.before; };
+  // whether the row has any of a thread's piece, and whether there may be a piece that it does not fill
+  auto has = [&](int i) { return kFull || (column(i) < width && (kLying != kZpCycled || column(i) + V > 0)); };
+  bool edge = false;
+#pragma unroll
+  for (int i = 0; i < M && kLying != kZpAligned; ++i) edge = edge || (has(i) && (column(i) < 0 || column(i) + V > width));
   float2 w[kHeld ? M : 1][H], gw[M][H], gb[M][H];
 #pragma unroll
   for (int i = 0; i < M; ++i) {
@@ -65,40 +63,40 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   const ZpPhiloxKey<false> key = drops ? zp_philox_key<false>(c.drop.state) : ZpPhiloxKey<false>{};
   const uint32_t limit = zp_drop_limit(c.drop.threshold);
   const float inv_w = 1.f / (float)width;
-  const int64_t row_bytes = c.width * (int64_t)sizeof(T);
+  const int64_t row_bytes = c.width * (int64_t)sizeof(T), next = own.next * row_bytes;
   float next_mean[R], next_rstd[R];
-  const float *mean_at = c.mean_in + first, *rstd_at = c.rstd_in + first;
+  const float *mean_at = c.mean_in + own.first, *rstd_at = c.rstd_in + own.first;
   auto load_stats = [&](int turn) {
 #pragma unroll
     for (int j = 0; j < R; ++j)
-      if (turn < n[j]) {
-        next_mean[j] = mean_at[j];
-        next_rstd[j] = rstd_at[j];
+      if (turn < own.n[j]) {
+        next_mean[j] = mean_at[j * own.next];
+        next_rstd[j] = rstd_at[j * own.next];
       }
-    mean_at += step;
-    rstd_at += step;
+    mean_at += own.step;
+    rstd_at += own.step;
   };
 #pragma unroll
   for (int j = 0; j < R; ++j) next_mean[j] = next_rstd[j] = 0.f;
   load_stats(0);
-  int64_t out = first * row_bytes;             // of the rows that are worked on, in every result
+  int64_t out = own.first * row_bytes - own.before * (int)sizeof(T);        // of the rows that are worked on, in every result
   uint32_t slots = ring, behind = ring + (stages - 1) * stage_bytes;
-  for (int turn = 0; turn < turns; ++turn) {
+  for (int turn = 0; turn < own.turns; ++turn) {
     float mean[R], rstd[R], s[2 * R];
 #pragma unroll
     for (int j = 0; j < R; ++j) { mean[j] = next_mean[j]; rstd[j] = next_rstd[j]; }
     zp_copy_wait(stages);
-    if (!kAligned) t.sync();                   // others' pieces are there; the last rows have been read
+    if (kLying == kZpShifted) t.sync();                   // others' pieces are there; the last rows have been read
     fetch(turn + stages - 1, behind);
     load_stats(turn + 1);
     float2 z[kHeld ? R : 1][M][H], g[kHeld ? R : 1][M][H];
     // z and gy w of row j, piece i, from the slots
     auto load = [&](int j, int i, float2 (&zz)[H], float2 (&gy)[H]) {
-      zp_read<T, kAligned>(t, slots + j * row_slots, sx.place_of(j), i, zz);
-      zp_read<T, kAligned>(t, slots + j * row_slots + p.slot, sy.place_of(j), i, gy);
-      if (!kAligned && tail && column(i) + tail == width) {
-        zp_cut<T>(tail, zz);
-        zp_cut<T>(tail, gy);
+      zp_read<T, kLying>(t, slots + j * row_slots, sx.place_of(j), i, zz);
+      zp_read<T, kLying>(t, slots + j * row_slots + p.slot, sy.place_of(j), i, gy);
+      if (kLying != kZpAligned && edge) {      // (a neighbour's elements, or nothing's)
+        zp_cut<T>(column(i), width, zz);
+        zp_cut<T>(column(i), width, gy);
       }
       const float2 minus = make_float2(-mean[j], -mean[j]), by = make_float2(rstd[j], rstd[j]);
 #pragma unroll
@@ -109,7 +107,7 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       float2 s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (turn >= n[j] || (!kFull && column(i) >= width)) continue;
+        if (turn >= own.n[j] || !has(i)) continue;
         float2 (&zz)[H] = z[kHeld ? j : 0][i], (&gz)[H] = g[kHeld ? j : 0][i];
         load(j, i, zz, gz);
         float2 ww[H];
@@ -126,20 +124,20 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       s[2 * j] = s1.x + s1.y;
       s[2 * j + 1] = s2.x + s2.y;
     }
-    t.sum(s, turn, !kAligned);
+    t.sum(s, turn, kLying == kZpShifted);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      ZpKept<T, kAligned, false, E> kept;
-      if (drops) kept.find(t, key, limit, turn < n[j] ? first + turn * step + j : 0, width, bytes);
+      ZpKept<T, kLying, false, E> kept;
+      if (drops) kept.find(t, key, limit, turn < own.n[j] ? own.first + turn * own.step + j * own.next : 0, width, bytes);
       const float2 minus1 = make_float2(-s[2 * j] * inv_w, -s[2 * j] * inv_w);
       const float2 minus2 = make_float2(-s[2 * j + 1] * inv_w, -s[2 * j + 1] * inv_w);
       const float2 by = make_float2(rstd[j], rstd[j]);
       const uint32_t slot = slots + j * row_slots;
-      const int64_t at = out + j * row_bytes;
+      const int64_t at = out + j * next;
       const uint32_t to = kHeld ? slot : results;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (turn >= n[j] || (!kFull && column(i) >= width)) continue;
+        if (turn >= own.n[j] || !has(i)) continue;
         float2 o[H], q[H];
         if constexpr (kHeld) {
 #pragma unroll
@@ -154,27 +152,27 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
             o[k] = __fmul2_rn(__ffma2_rn(zz[k], minus2, __ffma2_rn(q[k], ww[k], minus1)), by);
         }
         if constexpr (!kJoin) {
-          if (c.dx) zp_write<T, kAligned>(t, static_cast<char *>(c.dx) + at, to, i, o);
+          if (c.dx) zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, to, i, column(i), width, edge, o);
           continue;
         }
         if (third) {
-          zp_read<T, kAligned>(t, slot + 2 * p.slot, ss.place_of(j), i, q);
+          zp_read<T, kLying>(t, slot + 2 * p.slot, ss.place_of(j), i, q);
 #pragma unroll
           for (int k = 0; k < H; ++k) o[k] = __fadd2_rn(o[k], q[k]);
         }
-        if (c.dres) zp_write<T, kAligned>(t, static_cast<char *>(c.dres) + at, to, i, o);
+        if (c.dres) zp_write<T, kLying>(t, static_cast<char *>(c.dres) + at, to, i, column(i), width, edge, o);
         if (!c.dx) continue;
 #pragma unroll
         for (int k = 0; k < H && drops; ++k) o[k] = kept.drop(o[k], i, k, limit, c.drop.scale);
-        zp_write<T, kAligned>(t, static_cast<char *>(c.dx) + at, c.dres ? to + p.slot : to, i, o);
+        zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, c.dres ? to + p.slot : to, i, column(i), width, edge, o);
       }
     }
-    if constexpr (!kAligned) {
+    if constexpr (kLying == kZpShifted) {
       t.sync();
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        if (turn >= n[j]) continue;
-        const int64_t at = out + j * row_bytes;
+        if (turn >= own.n[j]) continue;
+        const int64_t at = out + j * next;
         const uint32_t from = kHeld ? slots + j * row_slots : results;
         if (kJoin && c.dres) zp_store_row<T, M>(t, static_cast<char *>(c.dres) + at, from, width);
         if (c.dx) zp_store_row<T, M>(t, static_cast<char *>(c.dx) + at, kJoin && c.dres ? from + p.slot : from, width);
@@ -183,14 +181,16 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       sy.advance();
       ss.advance();
     }
-    out += step * row_bytes;
+    out += own.step * row_bytes;
     behind = slots;
     slots = slots + stage_bytes == ring + ring_bytes ? ring : slots + stage_bytes;
   }
   zp_copy_wait(2);
   if (!c.partial) return;
-  // teams within a warp first, then those of the block (`copies` of them) through shared memory, in order
-  for (int o = t.size; o < 32; o <<= 1) {
+  // The teams' sums through shared memory, in order; of aligned rows those within a warp first, which have the same
+  // columns (of cycled rows each class has its own)
+  constexpr bool kByWarp = kLying != kZpCycled;
+  for (int o = t.size; kByWarp && o < 32; o <<= 1) {
 #pragma unroll
     for (int i = 0; i < M; ++i)
 #pragma unroll
@@ -202,16 +202,22 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       }
   }
   float *const all = reinterpret_cast<float *>(rings);           // [copies][2][row]
-  const int row = t.size * E, copies = t.walkers;
+  const int row = t.size * E, copies = kByWarp ? t.walkers : kZpTeamThreads / t.size;
   __syncthreads();                                               // the rings are done with
-  if (t.sub == 0) {
-    float *const mine = all + (size_t)t.walker * 2 * row;
+  if (!kByWarp || t.sub == 0) {
+    float *const mine = all + (size_t)(kByWarp ? t.walker : t.index) * 2 * row;
 #pragma unroll
     for (int i = 0; i < M; ++i)
 #pragma unroll
       for (int k = 0; k < H; ++k) {
-        *reinterpret_cast<float2 *>(mine + column(i) + 2 * k) = gw[i][k];
-        *reinterpret_cast<float2 *>(mine + row + column(i) + 2 * k) = gb[i][k];
+        const int at = column(i) + 2 * k;
+        if constexpr (kByWarp) {
+          *reinterpret_cast<float2 *>(mine + at) = gw[i][k];
+          *reinterpret_cast<float2 *>(mine + row + at) = gb[i][k];
+        } else {
+          if ((unsigned)at < (unsigned)width) { mine[at] = gw[i][k].x; mine[row + at] = gb[i][k].x; }
+          if ((unsigned)(at + 1) < (unsigned)width) { mine[at + 1] = gw[i][k].y; mine[row + at + 1] = gb[i][k].y; }
+        }
       }
   }
   __syncthreads();
@@ -226,38 +232,36 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
 
 bool is_join(const ZpNormCall &c) { return c.dsum || c.dres || c.drop.state; }
 
-template <typename T, bool kAligned, bool kFull, int E, int R, bool kJoin>
+template <typename T, int kLying, bool kFull, int E, int R, bool kJoin>
 int launch(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
   static ZpSmemOptIn opt_in;
-  if (int rc = zp_ensure_smem(norm_bwd_team_kernel<T, kAligned, kFull, E, R, kJoin>, p.smem, opt_in)) return rc;
-  zp_launch(norm_bwd_team_kernel<T, kAligned, kFull, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
+  if (int rc = zp_ensure_smem(norm_bwd_team_kernel<T, kLying, kFull, E, R, kJoin>, p.smem, opt_in)) return rc;
+  zp_launch(norm_bwd_team_kernel<T, kLying, kFull, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
   ZP_LAUNCH_CHECK("norm_bwd_team_kernel");
   return ZP_OK;
 }
-template <typename T, bool kAligned, bool kFull, bool kJoin>
+template <typename T, int kLying, bool kFull, bool kJoin>
 int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if constexpr (kAligned || !kJoin)
-    if (p.rows == 2) return launch<T, kAligned, kFull, 8, 2, kJoin>(c, p, st);
-  if (p.elements == 8) return launch<T, kAligned, kFull, 8, 1, kJoin>(c, p, st);
-  return p.elements == 16 ? launch<T, kAligned, kFull, 16, 1, kJoin>(c, p, st) : launch<T, kAligned, kFull, 32, 1, kJoin>(c, p, st);
+  if constexpr (kLying != kZpShifted || !kJoin)
+    if (p.rows == 2) return launch<T, kLying, kFull, 8, 2, kJoin>(c, p, st);
+  if (p.elements == 8) return launch<T, kLying, kFull, 8, 1, kJoin>(c, p, st);
+  return p.elements == 16 ? launch<T, kLying, kFull, 16, 1, kJoin>(c, p, st)
+                          : launch<T, kLying, kFull, 32, 1, kJoin>(c, p, st);
 }
-template <typename T, bool kJoin> int by_alignment(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (p.full) return by_elements<T, true, true, kJoin>(c, p, st);
-  return p.aligned ? by_elements<T, true, false, kJoin>(c, p, st) : by_elements<T, false, false, kJoin>(c, p, st);
+template <typename T, bool kJoin> int by_lying(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+  if (p.full) return by_elements<T, kZpAligned, true, kJoin>(c, p, st);
+  if (p.lying == kZpAligned) return by_elements<T, kZpAligned, false, kJoin>(c, p, st);
+  return p.lying == kZpCycled ? by_elements<T, kZpCycled, false, kJoin>(c, p, st)
+                              : by_elements<T, kZpShifted, false, kJoin>(c, p, st);
 }
 template <typename T> int by_kind(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  return is_join(c) ? by_alignment<T, true>(c, p, st) : by_alignment<T, false>(c, p, st);
+  return is_join(c) ? by_lying<T, true>(c, p, st) : by_lying<T, false>(c, p, st);
 }
 
 }  // namespace
 
 int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_t st) {
-  const size_t size = c.dtype == ZP_F32 ? 4 : 2;
-  const bool aligned = (c.width * size) % 16 == 0 && zp_piece_aligned(c.x, c.ldx, size) &&
-                       zp_piece_aligned(c.dy, c.ldy, size) && (!c.dsum || zp_piece_aligned(c.dsum, c.lds, size)) &&
-                       (!c.dx || zp_piece_aligned(c.dx, c.width, size)) &&
-                       (!c.dres || zp_piece_aligned(c.dres, c.width, size)) &&
-                       (!c.drop.state || c.width % 8 == 0);
+  const int lying = zp_lying(c, {{c.x, c.ldx}, {c.dy, c.ldy}, {c.dsum, c.lds}, {c.dx, c.width}, {c.dres, c.width}});
   const int64_t each = c.rows * c.width / ((int64_t)148 * kZpTeamThreads);       // elements a thread
   const int arrays = c.dsum ? 3 : 2;
   const bool join = is_join(c);
@@ -265,14 +269,14 @@ int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_
   // Two rows at a time, as in the forward: 16384 x 4096 bf16 93 us -> 76, joined 153 -> 132, 400000 x 32 23 -> 20.
   // Joined rows of a warp or less (60000 x 128 fp32 29 -> 31) or that are not aligned (30011 x 1001 fp16 150 -> 185:
   // registers) are better one by one.
-  const bool two = each >= 32 && (!join || (aligned && c.width > 256));
+  const bool two = each >= 32 && (!join || (lying != kZpShifted && c.width > 256));
   // (rows of many elements are read twice, so that their results cannot pass through the slots they came in)
-  const int results = aligned ? 0 : c.dx && c.dres ? 2 : 1;
+  const int results = lying != kZpShifted ? 0 : c.dx && c.dres ? 2 : 1;
   ZpTeamPlan p;
-  taken = c.dy && ((two && zp_team_plan(c, aligned, arrays, 0, last, 8, 2, p)) ||
-                   zp_team_plan(c, aligned, arrays, 0, last, 8, 1, p) ||
-                   zp_team_plan(c, aligned, arrays, 0, last, 16, 1, p) ||
-                   zp_team_plan(c, aligned, arrays, results, last, 32, 1, p));
+  taken = c.dy && ((two && zp_team_plan(c, lying, arrays, 0, last, 8, 2, p)) ||
+                   zp_team_plan(c, lying, arrays, 0, last, 8, 1, p) ||
+                   zp_team_plan(c, lying, arrays, 0, last, 16, 1, p) ||
+                   zp_team_plan(c, lying, arrays, results, last, 32, 1, p));
   if (!taken) return ZP_OK;
   parts = (int)p.blocks;
   if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);

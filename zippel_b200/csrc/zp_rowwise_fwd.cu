@@ -8,7 +8,7 @@
 namespace {
 
 // E elements of a thread in each of R rows at a time
-template <typename T, bool kAligned, bool kFull, int E, int R, bool kJoin>
+template <typename T, int kLying, bool kFull, int E, int R, bool kJoin>
 __global__ void __launch_bounds__(kZpTeamThreads, 1)
 norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant__ ZpTeamPlan p) {
   zp_after_previous();
@@ -21,21 +21,15 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   uint8_t *const bytes = reinterpret_cast<uint8_t *>(after_red) + t.index * p.bytes;
   const uint32_t stage_bytes = A * R * p.slot, ring_bytes = stages * stage_bytes;
   const uint32_t ring = zp_shared(after_red) + p.bytes * (kZpTeamThreads / p.team) + t.index * ring_bytes;
-  // a walker takes R rows after one another of each of its teams
-  const int64_t step = (int64_t)gridDim.x * t.walkers * t.per * R;
-  const int64_t first = (((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per + t.sub) * R;
-  ZpSource<kAligned> sx(t, c.x, c.ldx, c.rows, c.width, sizeof(T), first, step);
-  ZpSource<kAligned> sr(t, c.res, c.ldr, c.rows, c.width, sizeof(T), first, step);
-  int n[R];                                    // turns in which this team has its row j
-#pragma unroll
-  for (int j = 0; j < R; ++j) n[j] = zp_steps(c.rows, first + j, step);
-  const int turns = zp_steps(c.rows, first - t.sub * R, step);        // (a warp's teams go on together)
+  const ZpTeamRows<kLying, R> own(t, c.rows, width, p.cycle);
+  ZpSource<kLying> sx(t, c.x, c.ldx, c.rows, c.width, sizeof(T), own);
+  ZpSource<kLying> sr(t, c.res, c.ldr, c.rows, c.width, sizeof(T), own);
   auto fetch = [&](int turn, uint32_t to) {
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      if (turn >= n[j]) continue;
-      zp_fetch_row<T, kAligned, kFull, M>(t, to + j * A * p.slot, sx, j, width);
-      if (kJoin) zp_fetch_row<T, kAligned, kFull, M>(t, to + (j * A + 1) * p.slot, sr, j, width);
+      if (turn >= own.n[j]) continue;
+      zp_fetch_row<T, kLying, kFull, M>(t, to + j * A * p.slot, sx, j, width, own.before);
+      if (kJoin) zp_fetch_row<T, kLying, kFull, M>(t, to + (j * A + 1) * p.slot, sr, j, width, own.before);
     }
     sx.row += sx.step;
     if (kJoin) sr.row += sr.step;
@@ -43,48 +37,51 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   };
   for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
 
-  const int tail = kAligned ? 0 : zp_tail<T>(t, width);
   const bool wide = c.param_dtype == ZP_F32;
-  auto column = [&](int i) { return (t.lane + i * t.size) * V; };
+  auto column = [&](int i) { return (t.lane + i * t.size) * V - own.before; };
+  // whether the row has any of a thread's piece, and whether there may be a piece that it does not fill
+  auto has = [&](int i) { return kFull || (column(i) < width && (kLying != kZpCycled || column(i) + V > 0)); };
+  bool edge = false;
+#pragma unroll
+  for (int i = 0; i < M && kLying != kZpAligned; ++i) edge = edge || (has(i) && (column(i) < 0 || column(i) + V > width));
   float2 w[kHeld ? M : 1][H], b[kHeld ? M : 1][H];
 #pragma unroll
   for (int i = 0; i < (kHeld ? M : 0); ++i) {
     zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, w[i]);
     zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, b[i]);
   }
-  const bool drops = kJoin && c.drop.state;
   auto cut = [&](float2 (&v)[M][H]) {
-    if (kAligned || tail == 0) return;
+    if (kLying == kZpAligned || !edge) return;
 #pragma unroll
-    for (int i = 0; i < M; ++i)
-      if (column(i) + tail == width) zp_cut<T>(tail, v[i]);
+    for (int i = 0; i < M; ++i) zp_cut<T>(column(i), width, v[i]);
   };
+  const bool drops = kJoin && c.drop.state;
   const ZpPhiloxKey<false> key = drops ? zp_philox_key<false>(c.drop.state) : ZpPhiloxKey<false>{};
   const uint32_t limit = zp_drop_limit(c.drop.threshold);
   const float inv_w = 1.f / (float)width;
-  const int64_t row_bytes = c.width * (int64_t)sizeof(T);
-  int64_t out = first * row_bytes;             // of the rows that are worked on, in every result
+  const int64_t row_bytes = c.width * (int64_t)sizeof(T), next = own.next * row_bytes;
+  int64_t out = own.first * row_bytes - own.before * (int)sizeof(T);        // of the rows that are worked on, in every result
   uint32_t slots = ring, behind = ring + (stages - 1) * stage_bytes;
-  for (int turn = 0; turn < turns; ++turn) {
+  for (int turn = 0; turn < own.turns; ++turn) {
     zp_copy_wait(stages);
-    if (!kAligned) t.sync();                   // others' pieces are there; the last rows have been read
+    if (kLying == kZpShifted) t.sync();                   // others' pieces are there; the last rows have been read
     fetch(turn + stages - 1, behind);
     float2 v[R][M][H];
     float s[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const bool mine = turn < n[j];
+      const bool mine = turn < own.n[j];
       const uint32_t x = slots + j * A * p.slot, res = x + p.slot;
-      ZpKept<T, kAligned, kAligned, E> kept;
-      if (drops) kept.find(t, key, limit, mine ? first + turn * step + j : 0, width, bytes);
+      ZpKept<T, kLying, kLying != kZpShifted, E> kept;
+      if (drops) kept.find(t, key, limit, mine ? own.first + turn * own.step + j * own.next : 0, width, bytes);
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (!mine || (!kFull && column(i) >= width)) continue;
-        zp_read<T, kAligned>(t, x, sx.place_of(j), i, v[j][i]);
+        if (!mine || !has(i)) continue;
+        zp_read<T, kLying>(t, x, sx.place_of(j), i, v[j][i]);
         if constexpr (kJoin) {
           float2 q[H];
-          zp_read<T, kAligned>(t, res, sr.place_of(j), i, q);
+          zp_read<T, kLying>(t, res, sr.place_of(j), i, q);
 #pragma unroll
           for (int k = 0; k < H; ++k) {
             const float2 f = drops ? kept.drop(v[j][i][k], i, k, limit, c.drop.scale) : v[j][i][k];
@@ -92,21 +89,21 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
           }
           // rounded: what follows works on the sum as it is returned
           const uint4 packed = zp_pack<T>(v[j][i]);
-          if (kAligned)
-            reinterpret_cast<uint4 *>(static_cast<char *>(c.sum) + out + j * row_bytes)[t.lane + i * t.size] = packed;
           zp_unpack<T>(packed, v[j][i]);
+          if (kLying != kZpShifted)
+            zp_write<T, kLying>(t, static_cast<char *>(c.sum) + out + j * next, 0, i, column(i), width, edge, v[j][i]);
         }
       }
       cut(v[j]);
 #pragma unroll
       for (int i = 0; i < M; ++i)
-        if (mine && (kFull || column(i) < width)) {
+        if (mine && has(i)) {
 #pragma unroll
           for (int k = 0; k < H; ++k) sum = __fadd2_rn(sum, v[j][i][k]);
         }
       s[j] = sum.x + sum.y;
     }
-    t.sum(s, 0, !kAligned);
+    t.sum(s, 0, kLying == kZpShifted);
     float q[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
@@ -115,30 +112,30 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       const float2 minus = make_float2(-s[j], -s[j]);
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (turn >= n[j] || (!kFull && column(i) >= width)) continue;
-        if constexpr (kJoin && !kAligned)      // (the team has read all of this slot)
-          zp_write<T, kAligned>(t, nullptr, slots + j * A * p.slot, i, v[j][i]);
+        if (turn >= own.n[j] || !has(i)) continue;
+        if constexpr (kJoin && kLying == kZpShifted)      // (the team has read all of this slot)
+          zp_write<T, kLying>(t, nullptr, slots + j * A * p.slot, i, 0, 0, false, v[j][i]);
 #pragma unroll
         for (int k = 0; k < H; ++k) v[j][i][k] = __fadd2_rn(v[j][i][k], minus);
       }
       cut(v[j]);
 #pragma unroll
       for (int i = 0; i < M; ++i)
-        if (turn < n[j] && (kFull || column(i) < width)) {
+        if (turn < own.n[j] && has(i)) {
 #pragma unroll
           for (int k = 0; k < H; ++k) sq = __ffma2_rn(v[j][i][k], v[j][i][k], sq);
         }
       q[j] = sq.x + sq.y;
     }
-    t.sum(q, 1, !kAligned);
+    t.sum(q, 1, kLying == kZpShifted);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       const float rstd = rsqrtf(q[j] * inv_w + c.eps);
       const float2 both = make_float2(rstd, rstd);
-      char *const y = static_cast<char *>(c.y) + out + j * row_bytes;
+      char *const y = static_cast<char *>(c.y) + out + j * next;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (turn >= n[j] || (!kFull && column(i) >= width)) continue;
+        if (turn >= own.n[j] || !has(i)) continue;
         float2 ww[H], bb[H];
         if constexpr (!kHeld) {
           zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, ww);
@@ -148,66 +145,64 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
         for (int k = 0; k < H; ++k)
           v[j][i][k] = __ffma2_rn(__fmul2_rn(v[j][i][k], both), kHeld ? w[kHeld ? i : 0][k] : ww[k],
                                   kHeld ? b[kHeld ? i : 0][k] : bb[k]);
-        zp_write<T, kAligned>(t, y, slots + (j * A + A - 1) * p.slot, i, v[j][i]);
+        zp_write<T, kLying>(t, y, slots + (j * A + A - 1) * p.slot, i, column(i), width, edge, v[j][i]);
       }
-      if (t.lane == 0 && c.mean && turn < n[j]) {
-        const int64_t r = first + turn * step + j;
+      if (t.lane == 0 && c.mean && turn < own.n[j]) {
+        const int64_t r = own.first + turn * own.step + j * own.next;
         c.mean[r] = s[j];
         c.rstd[r] = rstd;
       }
     }
-    if constexpr (!kAligned) {
+    if constexpr (kLying == kZpShifted) {
       t.sync();
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        if (turn >= n[j]) continue;
-        const int64_t at = out + j * row_bytes;
+        if (turn >= own.n[j]) continue;
+        const int64_t at = out + j * next;
         zp_store_row<T, M>(t, static_cast<char *>(c.y) + at, slots + (j * A + A - 1) * p.slot, width);
         if (kJoin) zp_store_row<T, M>(t, static_cast<char *>(c.sum) + at, slots + j * A * p.slot, width);
       }
       sx.advance();
       sr.advance();
     }
-    out += step * row_bytes;
+    out += own.step * row_bytes;
     behind = slots;
     slots = slots + stage_bytes == ring + ring_bytes ? ring : slots + stage_bytes;
   }
   zp_copy_wait(2);
 }
 
-template <typename T, bool kAligned, bool kFull, int E, int R, bool kJoin>
+template <typename T, int kLying, bool kFull, int E, int R, bool kJoin>
 int launch(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
   static ZpSmemOptIn opt_in;
-  if (int rc = zp_ensure_smem(norm_fwd_team_kernel<T, kAligned, kFull, E, R, kJoin>, p.smem, opt_in)) return rc;
-  zp_launch(norm_fwd_team_kernel<T, kAligned, kFull, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
+  if (int rc = zp_ensure_smem(norm_fwd_team_kernel<T, kLying, kFull, E, R, kJoin>, p.smem, opt_in)) return rc;
+  zp_launch(norm_fwd_team_kernel<T, kLying, kFull, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
   ZP_LAUNCH_CHECK("norm_fwd_team_kernel");
   return ZP_OK;
 }
-template <typename T, bool kAligned, bool kFull, bool kJoin>
+template <typename T, int kLying, bool kFull, bool kJoin>
 int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (p.elements == 8) return launch<T, kAligned, kFull, 8, 1, kJoin>(c, p, st);
-  if (p.elements == 32) return launch<T, kAligned, kFull, 32, 1, kJoin>(c, p, st);
+  if (p.elements == 8) return launch<T, kLying, kFull, 8, 1, kJoin>(c, p, st);
+  if (p.elements == 32) return launch<T, kLying, kFull, 32, 1, kJoin>(c, p, st);
   if constexpr (sizeof(T) == 2)
-    if (p.rows == 2) return launch<T, kAligned, kFull, 16, 2, kJoin>(c, p, st);
-  return launch<T, kAligned, kFull, 16, 1, kJoin>(c, p, st);
+    if (p.rows == 2) return launch<T, kLying, kFull, 16, 2, kJoin>(c, p, st);
+  return launch<T, kLying, kFull, 16, 1, kJoin>(c, p, st);
 }
-template <typename T, bool kJoin> int by_alignment(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (p.full) return by_elements<T, true, true, kJoin>(c, p, st);
-  return p.aligned ? by_elements<T, true, false, kJoin>(c, p, st) : by_elements<T, false, false, kJoin>(c, p, st);
+template <typename T, bool kJoin> int by_lying(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+  if (p.full) return by_elements<T, kZpAligned, true, kJoin>(c, p, st);
+  if (p.lying == kZpAligned) return by_elements<T, kZpAligned, false, kJoin>(c, p, st);
+  return p.lying == kZpCycled ? by_elements<T, kZpCycled, false, kJoin>(c, p, st)
+                              : by_elements<T, kZpShifted, false, kJoin>(c, p, st);
 }
 template <typename T> int by_kind(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  return c.res ? by_alignment<T, true>(c, p, st) : by_alignment<T, false>(c, p, st);
+  return c.res ? by_lying<T, true>(c, p, st) : by_lying<T, false>(c, p, st);
 }
 
 }  // namespace
 
 int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
   const size_t size = c.dtype == ZP_F32 ? 4 : 2;
-  // (results lie row behind row; the counters of dropout go by eight elements)
-  const bool aligned = (c.width * size) % 16 == 0 && zp_piece_aligned(c.x, c.ldx, size) &&
-                       zp_piece_aligned(c.y, c.width, size) &&
-                       (!c.res || (zp_piece_aligned(c.res, c.ldr, size) && zp_piece_aligned(c.sum, c.width, size))) &&
-                       (!c.drop.state || c.width % 8 == 0);
+  const int lying = zp_lying(c, {{c.x, c.ldx}, {c.y, c.width}, {c.res, c.ldr}, {c.sum, c.width}});
   // Two rows at a time halve what joining the sums of a team of several warps costs (16384 x 4096 bf16 59 us ->
   // 49), and leave the ring fewer stages (fp32 42 -> 50, joined without dropout 92 -> 99) and the blocks fewer
   // turns to share out (60000 x 128 bf16 9.5 -> 10.4).  Few elements are spread over more threads.
@@ -215,10 +210,10 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
   const int arrays = c.res ? 2 : 1;
   const bool two = each >= 64 && c.width > 512 && size == 2 && (!c.res || c.drop.state);
   ZpTeamPlan p;
-  taken = (two && zp_team_plan(c, aligned, arrays, 0, 0, 16, 2, p)) ||
-          (each >= 32 && zp_team_plan(c, aligned, arrays, 0, 0, 16, 1, p)) ||
-          zp_team_plan(c, aligned, arrays, 0, 0, 8, 1, p) || zp_team_plan(c, aligned, arrays, 0, 0, 16, 1, p) ||
-          zp_team_plan(c, aligned, arrays, 0, 0, 32, 1, p);
+  taken = (two && zp_team_plan(c, lying, arrays, 0, 0, 16, 2, p)) ||
+          (each >= 32 && zp_team_plan(c, lying, arrays, 0, 0, 16, 1, p)) ||
+          zp_team_plan(c, lying, arrays, 0, 0, 8, 1, p) || zp_team_plan(c, lying, arrays, 0, 0, 16, 1, p) ||
+          zp_team_plan(c, lying, arrays, 0, 0, 32, 1, p);
   if (!taken) return ZP_OK;
   if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);
   if (c.dtype == ZP_F16) return by_kind<__half>(c, p, st);
