@@ -195,7 +195,7 @@ def test_rows_that_lie_elsewhere(width, kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("width", [12, 100, 1002, 5001, 8186, 8190, 9999, 16377])
+@pytest.mark.parametrize("width", [12, 100, 1002, 4090, 5001, 8186, 8190, 9999, 12288, 16377, 32768, 33001])
 def test_rows_that_share_pieces_of_memory(width, dtype):
     """Widths that eight does not divide, of every class modulo eight, row behind row and from an odd address, few
     rows (fewer than a cycle of eight) and more than there are blocks: gradients of the join with dropout."""

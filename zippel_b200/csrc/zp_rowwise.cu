@@ -166,8 +166,8 @@ __device__ __forceinline__ float param(const P *w, int64_t c, float otherwise) {
   return w ? zp_float(w[c]) : otherwise;
 }
 
-// Rows that no team's shared memory holds (above 16384 elements, or where the ring would have one stage):
-// one block per row, passes over global memory.
+// Rows that no team holds (above 65536 elements, 32768 in the backward; shifted ones above 8192): one block
+// per row, passes over global memory.
 template <typename T, typename P>
 __global__ void __launch_bounds__(kThreads)
 norm_fwd_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, const T *__restrict__ res,

@@ -1,6 +1,7 @@
 // Operators over the rows of a matrix: what their kernels share.
 //
-// A row is worked on by a team of 2 to 512 threads, E elements to a thread in pieces of 16 bytes; a team
+// A row is worked on by a team of 2 to 512 threads, or of a cluster of blocks of 512, E elements to a thread in
+// pieces of 16 bytes; a team
 // takes R rows at a time, so that what a row costs beside its elements (the joining of sums, barriers,
 // addresses) is shared.  Teams of a warp or less add up by shuffles, larger ones through shared memory and a
 // named barrier of their own.  Arithmetic on the elements goes by pairs (one instruction for two): these
@@ -137,16 +138,22 @@ __device__ __forceinline__ void zp_params(const void *w, bool wide, bool vectors
 constexpr int kZpTeamThreads = 512;            // of a block
 constexpr int kZpTeamWarps = kZpTeamThreads / 32;
 
+constexpr int kZpMostRanks = 8;                // blocks of a cluster
+// shared memory in front of the rings: room for two turns' sums of warps, and of blocks
+constexpr int kZpSumsBytes = sizeof(float) * 2 * 4 * (kZpTeamWarps + kZpMostRanks);
+
 // Where a thread stands.  A "walker" is what goes through rows by itself: a warp, with one or several
-// teams in it, or a team of several warps.
-struct ZpTeam {
-  int size, lane;                              // threads of a team, this one's place in it
+// teams in it, or a team of several warps.  kWide: the team is a cluster of blocks, each with pieces of its own
+// of every row.
+template <bool kWide> struct ZpTeam {
+  int size, lane;                              // threads of a team (in the block), this one's place among them
   int index;                                   // of the team in the block
   int per, sub;                                // teams of a walker, this one among them
   int walker, walkers;
-  float *red;                                  // [2][warps of the block][4], for teams of several warps
+  int ranks, rank;                             // blocks of the team, this one's place among them
+  float *red;                                  // [2][warps of the block][4], then [2][blocks][4]
 
-  __device__ __forceinline__ ZpTeam(int team_size, float *red_) {
+  __device__ __forceinline__ ZpTeam(int team_size, int blocks, float *red_) {
     size = team_size;
     const int tid = threadIdx.x, wide = size > 32 ? size : 32;
     lane = tid & (size - 1);
@@ -156,6 +163,21 @@ struct ZpTeam {
     walkers = kZpTeamThreads / wide;
     sub = index - walker * per;
     red = red_;
+    ranks = kWide ? blocks : 1;
+    rank = 0;
+    if constexpr (kWide) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  }
+  // number of this thread's piece i of a row, and the pieces from one to the next
+  __device__ __forceinline__ int piece(int i) const { return kWide ? lane + (i * ranks + rank) * size : lane + i * size; }
+  __device__ __forceinline__ int apart() const { return kWide ? ranks * size : size; }
+  __device__ __forceinline__ int64_t block() const { return kWide ? blockIdx.x / ranks : blockIdx.x; }
+  __device__ __forceinline__ int64_t blocks() const { return kWide ? gridDim.x / ranks : gridDim.x; }
+  // all blocks of the team; what they wrote in each other's shared memory is there
+  __device__ __forceinline__ void meet() const {
+    if constexpr (kWide) {
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
   }
   __device__ __forceinline__ void sync() const {
     if (size <= 32) __syncwarp();
@@ -214,6 +236,28 @@ struct ZpTeam {
 #pragma unroll
       for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, s, k * kOwn);
     }
+    if constexpr (kWide) {                     // the blocks' sums, added by each in the same order
+      float *const buf = red + 2 * 4 * kZpTeamWarps + (turn & 1) * (kZpMostRanks * 4);
+      if (lane < ranks * K) {
+        const int k = lane % K;
+        float one = v[0];
+#pragma unroll
+        for (int i = 1; i < K; ++i) one = k == i ? v[i] : one;
+        const uint32_t own = (uint32_t)__cvta_generic_to_shared(buf + rank * 4 + k);
+        uint32_t there;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(own), "r"(lane / K));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(one) : "memory");
+      }
+      meet();
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] = 0.f;
+      for (int b = 0; b < ranks; ++b) {
+        const float4 q = *reinterpret_cast<const float4 *>(buf + 4 * b);
+        const float each[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += each[k];
+      }
+    }
   }
 };
 
@@ -254,10 +298,11 @@ template <int kLying, int R> struct ZpTeamRows {
   int64_t first, step;
   int next, turns, before;
   int n[R];
-  __device__ __forceinline__ ZpTeamRows(const ZpTeam &t, int64_t rows, int width, int cycle_) {
+  template <bool kWide>
+  __device__ __forceinline__ ZpTeamRows(const ZpTeam<kWide> &t, int64_t rows, int width, int cycle_) {
     const int cycle = kLying == kZpCycled ? cycle_ : 1;
-    const int64_t teams = (int64_t)gridDim.x * t.walkers * t.per;             // a multiple of the cycle
-    const int64_t team = ((int64_t)t.walker * gridDim.x + blockIdx.x) * t.per;
+    const int64_t teams = t.blocks() * t.walkers * t.per;                    // a multiple of the cycle
+    const int64_t team = (t.walker * t.blocks() + t.block()) * t.per;
     auto first_of = [&](int64_t u) { return kLying == kZpCycled ? u % cycle + u / cycle * cycle * R : u * R; };
     first = first_of(team + t.sub);
     step = teams * R;
@@ -279,12 +324,12 @@ template <int kLying> struct ZpSource {
   const char *row, *begin, *end;
   int64_t step, next;                          // bytes from a team's rows to its next ones, and from row to row
   int place;                                   // within 16 bytes, of the first of the rows that are worked on
-  template <int R>
-  __device__ __forceinline__ ZpSource(const ZpTeam &t, const void *base, int64_t ld, int64_t rows, int64_t width,
+  template <bool kWide, int R>
+  __device__ __forceinline__ ZpSource(const ZpTeam<kWide> &t, const void *base, int64_t ld, int64_t rows, int64_t width,
                                       int size, const ZpTeamRows<kLying, R> &own) {
     begin = static_cast<const char *>(base);
     end = begin + ((rows - 1) * ld + width) * size;
-    row = begin + (own.first * ld - own.before) * size + (kShifted ? 0 : 16 * t.lane);
+    row = begin + (own.first * ld - own.before) * size + (kShifted ? 0 : 16 * t.piece(0));
     step = own.step * ld * size;
     next = own.next * ld * size;
     place = kShifted ? (int)(reinterpret_cast<uintptr_t>(row) & 15) : 0;
@@ -298,8 +343,8 @@ template <int kLying> struct ZpSource {
 // Row j of the next rows, `width` elements of T, into a slot.  Each thread copies its own pieces (kFull: it has
 // them all), so that the row begins `before` elements behind the slot's begin; shifted rows keep their place
 // within 16 bytes.
-template <typename T, int kLying, bool kFull, int M>
-__device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, uint32_t slot, const ZpSource<kLying> &s, int j,
+template <typename T, int kLying, bool kFull, int M, bool kWide>
+__device__ __forceinline__ void zp_fetch_row(const ZpTeam<kWide> &t, uint32_t slot, const ZpSource<kLying> &s, int j,
                                              int width, int before) {
   constexpr int V = kZpVec<T>;
   const char *const row = j ? s.row + j * s.next : s.row;
@@ -307,9 +352,9 @@ __device__ __forceinline__ void zp_fetch_row(const ZpTeam &t, uint32_t slot, con
     const uint32_t to = slot + 16 * t.lane;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
-      const int c = (t.lane + i * t.size) * V - before;
+      const int c = t.piece(i) * V - before;
       if (kFull || (c < width && (kLying == kZpAligned || c + V > 0))) {
-        const char *const from = row + 16 * i * t.size;
+        const char *const from = row + 16 * i * t.apart();
         if (kLying == kZpAligned || from + 16 <= s.end)
           zp_copy16(to + 16 * i * t.size, from);
         else                                   // the array's last piece: nothing is read behind its end
@@ -365,8 +410,8 @@ template <int kSize> __device__ __forceinline__ uint4 zp_read_between(uint32_t a
 }
 
 // Piece number i of a thread, of a row in a slot.
-template <typename T, int kLying>
-__device__ __forceinline__ void zp_read(const ZpTeam &t, uint32_t slot, int place, int i, float2 (&v)[kZpVec<T> / 2]) {
+template <typename T, int kLying, bool kWide>
+__device__ __forceinline__ void zp_read(const ZpTeam<kWide> &t, uint32_t slot, int place, int i, float2 (&v)[kZpVec<T> / 2]) {
   const uint32_t at = slot + 16 * (t.lane + i * t.size);
   zp_unpack<T>(kLying == kZpShifted ? zp_read_between<sizeof(T)>(at, place) : zp_lds16(at), v);
 }
@@ -381,12 +426,12 @@ template <typename T> __device__ __forceinline__ void zp_cut(int c, int width, f
 // Results, piece i from column c on.  `row`: where the team's first piece of the row goes; of a piece that the
 // row shares (`edge`: the thread may have one) its own elements alone are written.  Shifted rows go into a slot, 16
 // bytes from its start, from where zp_store_row takes them once the whole team has written.
-template <typename T, int kLying>
-__device__ __forceinline__ void zp_write(const ZpTeam &t, char *row, uint32_t slot, int i, int c, int width, bool edge,
+template <typename T, int kLying, bool kWide>
+__device__ __forceinline__ void zp_write(const ZpTeam<kWide> &t, char *row, uint32_t slot, int i, int c, int width, bool edge,
                                          const float2 (&v)[kZpVec<T> / 2]) {
-  const int q = t.lane + i * t.size;
+  const int q = t.piece(i);
   const uint4 packed = zp_pack<T>(v);
-  if constexpr (kLying == kZpShifted) {
+  if constexpr (kLying == kZpShifted) {        // (the rows of a block)
     zp_sts16(slot + 16 * q + 16, packed);
   } else if (kLying == kZpAligned || !edge || (c >= 0 && c + kZpVec<T> <= width)) {
     reinterpret_cast<uint4 *>(row)[q] = packed;
@@ -401,8 +446,8 @@ __device__ __forceinline__ void zp_write(const ZpTeam &t, char *row, uint32_t sl
     }
   }
 }
-template <typename T, int M>
-__device__ __forceinline__ void zp_store_row(const ZpTeam &t, char *row, uint32_t slot, int width) {
+template <typename T, int M, bool kWide>
+__device__ __forceinline__ void zp_store_row(const ZpTeam<kWide> &t, char *row, uint32_t slot, int width) {
   const int place = (int)(reinterpret_cast<uintptr_t>(row) & 15), end = place + width * (int)sizeof(T);
   char *const to = row - place;
   const uint32_t from = place ? slot : slot + 16;
@@ -448,7 +493,8 @@ template <typename T, int kLying, bool kWords, int E> struct ZpKept {
   uint32_t w[kWords ? E / 2 : 1];
 
   // (all threads of a warp come here together)
-  __device__ __forceinline__ void find(const ZpTeam &t, const ZpPhiloxKey<false> &key, uint32_t limit, int64_t r, int width,
+  template <bool kWide>
+  __device__ __forceinline__ void find(const ZpTeam<kWide> &t, const ZpPhiloxKey<false> &key, uint32_t limit, int64_t r, int width,
                                        uint8_t *bytes) {
     if constexpr (kLying != kZpShifted) {
       if (!kWords) w[0] = 0;
@@ -457,7 +503,7 @@ template <typename T, int kLying, bool kWords, int E> struct ZpKept {
 #pragma unroll
       for (int i = 0; i < E / 8; ++i) {
         // fp32: of pieces 2i and 2i + 1 the even lane works out the first one's counter, the odd one the other's
-        const int place = sizeof(T) == 2 ? t.lane + i * t.size : (t.lane + (2 * i + odd) * t.size) / 2;
+        const int place = sizeof(T) == 2 ? t.piece(i) : t.piece(2 * i + odd) / 2;
         uint4 q = zp_philox(key, first + place);
         if constexpr (kWords) {
           if constexpr (sizeof(T) == 4) {      // first half of a counter for the even lane
@@ -510,43 +556,98 @@ template <typename T, int kLying, bool kWords, int E> struct ZpKept {
 // lie, whether every thread has all its pieces, whether weight and bias lie in aligned ones, and the ring's sizes.
 struct ZpTeamPlan {
   int team, elements, rows;
+  int ranks;                                   // blocks of a team; above one it is a cluster
   int lying, cycle;                            // rows of a class are `cycle` apart
   bool full, vectors;
   int slot, bytes, stages;                     // bytes of a slot, of the counters' bits of a team
   size_t smem;
   unsigned blocks;
 };
-// `arrays` come in per row; `results`: slots of a row that results pass through besides those of the ring;
-// `last_per_element`: bytes of shared memory per element of a block's teams that
+// The largest number of teams up to `most` of which every class of the cycle has as many
+inline int64_t zp_whole_cycles(const ZpTeamPlan &p, int64_t most) {
+  const int teams = kZpTeamThreads / p.team;
+  const int64_t by = p.cycle > teams ? p.cycle / teams : 1;
+  return most / by * by;
+}
+// `arrays` come in per row; `last_per_element`: bytes of shared memory per element of a block's teams that
 // the kernel needs when the ring is done with.  False: this does not fit.
-inline bool zp_team_plan(const ZpNormCall &c, int lying, int arrays, int results, size_t last_per_element,
-                         int elements, int rows, ZpTeamPlan &p) {
+inline bool zp_team_plan(const ZpNormCall &c, int lying, int arrays, size_t last_per_element, int elements, int rows,
+                         ZpTeamPlan &p) {
   const int64_t size = c.dtype == ZP_F32 ? 4 : 2;
   const int64_t span = lying == kZpCycled ? c.width + 7 : c.width;             // elements of a row's pieces
-  if (span > (int64_t)kZpTeamThreads * elements) return false;
+  p.ranks = 1;
+  while (span > (int64_t)kZpTeamThreads * elements * p.ranks && p.ranks <= kZpMostRanks) p.ranks *= 2;
+  // (pieces of a shifted row that lie in two blocks would have to be put together across them)
+  if (p.ranks > kZpMostRanks || (p.ranks > 1 && lying == kZpShifted)) return false;
   p.lying = lying;
   p.cycle = lying != kZpCycled ? 1 : c.width % 2 ? 8 : c.width % 4 ? 4 : 2;
   p.vectors = lying != kZpCycled && c.width % (16 / size) == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0 &&
               reinterpret_cast<uintptr_t>(c.b) % 16 == 0;
   p.elements = elements;
   p.rows = rows;
-  const int64_t need = zp_ceil_div(span, elements);
+  const int64_t need = p.ranks > 1 ? kZpTeamThreads : zp_ceil_div(span, elements);
   for (p.team = 2; p.team < need; p.team *= 2) {}
-  p.full = lying == kZpAligned && (int64_t)p.team * elements == c.width;
+  p.full = lying == kZpAligned && (int64_t)p.team * elements * p.ranks == c.width;
   const int teams = kZpTeamThreads / p.team;
   p.slot = (int)(p.team * elements * size) + (lying == kZpShifted ? 48 : 0);
   p.bytes = lying != kZpShifted || !c.drop.state ? 0 : (int)zp_align_up((size_t)c.width / 8 + 3, 16);
-  const size_t red = sizeof(float) * 2 * 4 * kZpTeamWarps, fixed = red + (size_t)(p.bytes + results * p.slot) * teams;
+  const size_t fixed = kZpSumsBytes + (size_t)p.bytes * teams;
   const size_t last = last_per_element * kZpTeamThreads * elements, room = 226 * 1024;
   const size_t stage = (size_t)arrays * rows * p.slot * teams;
   p.stages = fixed + 4 * stage <= room ? 4 : fixed + 3 * stage <= room ? 3 : 2;
   if (fixed + p.stages * stage > room || fixed + last > room) return false;
-  p.smem = fixed + (p.stages * stage > last ? p.stages * stage : last);   // (results lie behind the ring)
-  const int64_t units = zp_ceil_div(c.rows, rows * (p.team < 32 ? 32 / p.team : 1));
-  // (classes of a cycle have as many teams each)
-  const int64_t by = p.cycle > teams ? p.cycle / teams : 1;
-  p.blocks = (unsigned)(units < 148 / by * by ? zp_ceil_div(units, by) * by : 148 / by * by);
+  p.smem = fixed + (p.stages * stage > last ? p.stages * stage : last);
+  const int64_t units = zp_ceil_div(c.rows, rows * (p.team < 32 ? 32 / p.team : 1)), all = 148 / p.ranks;
+  int64_t own = zp_whole_cycles(p, all);
+  if (units < own) {                           // as few as there is work for
+    const int64_t by = zp_whole_cycles(p, units);
+    own = by == units ? units : by + (p.cycle > teams ? p.cycle / teams : 1);
+  }
+  p.blocks = (unsigned)(own * p.ranks);
   return true;
+}
+// Clusters of `kernel` that run at the same time, looked up once per device and size
+struct ZpClusters {
+  std::mutex lock;
+  int most[64][4] = {};
+};
+template <typename Kernel> int zp_fit_clusters(Kernel kernel, ZpTeamPlan &p, ZpClusters &state) {
+  int dev = 0, log = p.ranks == 2 ? 1 : p.ranks == 4 ? 2 : 3;
+  ZP_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return ZP_ERR_UNSUPPORTED;
+  std::lock_guard<std::mutex> hold(state.lock);
+  int &most = state.most[dev][log];
+  if (most == 0) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.ranks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(148 / p.ranks * p.ranks); cfg.blockDim = dim3(kZpTeamThreads); cfg.dynamicSmemBytes = 227 * 1024;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    ZP_CUDA(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg));
+    if (most < 8) return ZP_ERR_UNSUPPORTED;
+  }
+  if ((int64_t)p.blocks > (int64_t)most * p.ranks) p.blocks = (unsigned)(zp_whole_cycles(p, most) * p.ranks);
+  return ZP_OK;
+}
+// One kernel of teams; kWide: teams are clusters
+template <bool kWide, typename Kernel>
+int zp_launch_teams(Kernel kernel, const char *name, const ZpNormCall &c, ZpTeamPlan &p, ZpSmemOptIn &opt_in,
+                    ZpClusters &clusters, cudaStream_t st) {
+  if (int rc = zp_ensure_smem(kernel, kWide ? 227 * 1024 : p.smem, opt_in)) return rc;
+  if constexpr (kWide)
+    if (int rc = zp_fit_clusters(kernel, p, clusters)) return rc;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.ranks; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.blocks); cfg.blockDim = dim3(kZpTeamThreads); cfg.dynamicSmemBytes = p.smem; cfg.stream = st;
+  cfg.attrs = attr; cfg.numAttrs = kWide ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, c, (const ZpTeamPlan)p);                       // errors: ZP_LAUNCH_CHECK
+  ZP_LAUNCH_CHECK(name);
+  return ZP_OK;
 }
 // How the rows of an array of a call lie; the call's are shifted where one array's are
 inline int zp_lying(const ZpNormCall &c, const void *p, int64_t ld) {

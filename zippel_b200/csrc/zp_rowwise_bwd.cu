@@ -8,23 +8,20 @@
 
 namespace {
 
-template <typename T, int kLying, bool kFull, int E, int R, bool kJoin>
+template <typename T, int kLying, bool kFull, int E, int R, bool kJoin, bool kWide>
 __global__ void __launch_bounds__(kZpTeamThreads, 1)
 norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant__ ZpTeamPlan p) {
   zp_after_previous();
   constexpr int V = kZpVec<T>, H = V / 2, M = E / V;
-  constexpr bool kHeld = E <= 16;              // the weight, z and gy w stay in registers
   extern __shared__ __align__(16) char smem[];
-  const ZpTeam t(p.team, reinterpret_cast<float *>(smem));
+  const ZpTeam<kWide> t(p.team, p.ranks, reinterpret_cast<float *>(smem));
   const int width = (int)c.width, stages = p.stages;
-  char *const after_red = smem + sizeof(float) * 2 * 4 * kZpTeamWarps;
+  char *const after_red = smem + kZpSumsBytes;
   uint8_t *const bytes = reinterpret_cast<uint8_t *>(after_red) + t.index * p.bytes;
   char *const rings = after_red + p.bytes * (kZpTeamThreads / p.team);
   const bool third = kJoin && c.dsum;          // of the arrays that come in
   const uint32_t row_slots = (third ? 3 : 2) * p.slot, stage_bytes = R * row_slots, ring_bytes = stages * stage_bytes;
   const uint32_t ring = zp_shared(rings) + t.index * ring_bytes;
-  const uint32_t results = zp_shared(rings) + (kZpTeamThreads / p.team) * ring_bytes +
-                           t.index * (c.dx && c.dres ? 2 : 1) * p.slot;              // behind the rings
   const ZpTeamRows<kLying, R> own(t, c.rows, width, p.cycle);
   ZpSource<kLying> sx(t, c.x, c.ldx, c.rows, c.width, sizeof(T), own);
   ZpSource<kLying> sy(t, c.dy, c.ldy, c.rows, c.width, sizeof(T), own);
@@ -46,16 +43,16 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
 
   const bool wide = c.param_dtype == ZP_F32;
-  auto column = [&](int i) { return (t.lane + i * t.size) * V - own.before; };
+  auto column = [&](int i) { return t.piece(i) * V - own.before; };
   // whether the row has any of a thread's piece, and whether there may be a piece that it does not fill
   auto has = [&](int i) { return kFull || (column(i) < width && (kLying != kZpCycled || column(i) + V > 0)); };
   bool edge = false;
 #pragma unroll
   for (int i = 0; i < M && kLying != kZpAligned; ++i) edge = edge || (has(i) && (column(i) < 0 || column(i) + V > width));
-  float2 w[kHeld ? M : 1][H], gw[M][H], gb[M][H];
+  float2 w[M][H], gw[M][H], gb[M][H];
 #pragma unroll
   for (int i = 0; i < M; ++i) {
-    if constexpr (kHeld) zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, w[i]);
+    zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, w[i]);
 #pragma unroll
     for (int k = 0; k < H; ++k) gw[i][k] = gb[i][k] = make_float2(0.f, 0.f);
   }
@@ -80,6 +77,7 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   for (int j = 0; j < R; ++j) next_mean[j] = next_rstd[j] = 0.f;
   load_stats(0);
   int64_t out = own.first * row_bytes - own.before * (int)sizeof(T);        // of the rows that are worked on, in every result
+  t.meet();                                    // the team's blocks run
   uint32_t slots = ring, behind = ring + (stages - 1) * stage_bytes;
   for (int turn = 0; turn < own.turns; ++turn) {
     float mean[R], rstd[R], s[2 * R];
@@ -89,36 +87,30 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     if (kLying == kZpShifted) t.sync();                   // others' pieces are there; the last rows have been read
     fetch(turn + stages - 1, behind);
     load_stats(turn + 1);
-    float2 z[kHeld ? R : 1][M][H], g[kHeld ? R : 1][M][H];
-    // z and gy w of row j, piece i, from the slots
-    auto load = [&](int j, int i, float2 (&zz)[H], float2 (&gy)[H]) {
-      zp_read<T, kLying>(t, slots + j * row_slots, sx.place_of(j), i, zz);
-      zp_read<T, kLying>(t, slots + j * row_slots + p.slot, sy.place_of(j), i, gy);
-      if (kLying != kZpAligned && edge) {      // (a neighbour's elements, or nothing's)
-        zp_cut<T>(column(i), width, zz);
-        zp_cut<T>(column(i), width, gy);
-      }
-      const float2 minus = make_float2(-mean[j], -mean[j]), by = make_float2(rstd[j], rstd[j]);
-#pragma unroll
-      for (int k = 0; k < H; ++k) zz[k] = __fmul2_rn(__fadd2_rn(zz[k], minus), by);
-    };
+    float2 z[R][M][H], g[R][M][H];             // normalised rows, and gy w
 #pragma unroll
     for (int j = 0; j < R; ++j) {
+      const float2 minus = make_float2(-mean[j], -mean[j]), by = make_float2(rstd[j], rstd[j]);
+      const uint32_t slot = slots + j * row_slots;
       float2 s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
         if (turn >= own.n[j] || !has(i)) continue;
-        float2 (&zz)[H] = z[kHeld ? j : 0][i], (&gz)[H] = g[kHeld ? j : 0][i];
-        load(j, i, zz, gz);
-        float2 ww[H];
-        if constexpr (!kHeld) zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, ww);
+        zp_read<T, kLying>(t, slot, sx.place_of(j), i, z[j][i]);
+        zp_read<T, kLying>(t, slot + p.slot, sy.place_of(j), i, g[j][i]);
+        if (kLying != kZpAligned && edge) {    // (a neighbour's elements, or nothing's)
+          zp_cut<T>(column(i), width, z[j][i]);
+          zp_cut<T>(column(i), width, g[j][i]);
+        }
 #pragma unroll
         for (int k = 0; k < H; ++k) {
-          gw[i][k] = __ffma2_rn(gz[k], zz[k], gw[i][k]);
-          gb[i][k] = __fadd2_rn(gb[i][k], gz[k]);
-          gz[k] = __fmul2_rn(gz[k], kHeld ? w[kHeld ? i : 0][k] : ww[k]);
-          s1 = __fadd2_rn(s1, gz[k]);
-          s2 = __ffma2_rn(gz[k], zz[k], s2);
+          const float2 zz = __fmul2_rn(__fadd2_rn(z[j][i][k], minus), by), gy = g[j][i][k], gz = __fmul2_rn(gy, w[i][k]);
+          gw[i][k] = __ffma2_rn(gy, zz, gw[i][k]);
+          gb[i][k] = __fadd2_rn(gb[i][k], gy);
+          s1 = __fadd2_rn(s1, gz);
+          s2 = __ffma2_rn(gz, zz, s2);
+          z[j][i][k] = zz;
+          g[j][i][k] = gz;
         }
       }
       s[2 * j] = s1.x + s1.y;
@@ -134,25 +126,15 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       const float2 by = make_float2(rstd[j], rstd[j]);
       const uint32_t slot = slots + j * row_slots;
       const int64_t at = out + j * next;
-      const uint32_t to = kHeld ? slot : results;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
         if (turn >= own.n[j] || !has(i)) continue;
         float2 o[H], q[H];
-        if constexpr (kHeld) {
 #pragma unroll
-          for (int k = 0; k < H; ++k)
-            o[k] = __fmul2_rn(__ffma2_rn(z[j][i][k], minus2, __fadd2_rn(g[j][i][k], minus1)), by);
-        } else {
-          float2 zz[H], ww[H];
-          load(j, i, zz, q);
-          zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, ww);
-#pragma unroll
-          for (int k = 0; k < H; ++k)
-            o[k] = __fmul2_rn(__ffma2_rn(zz[k], minus2, __ffma2_rn(q[k], ww[k], minus1)), by);
-        }
+        for (int k = 0; k < H; ++k)
+          o[k] = __fmul2_rn(__ffma2_rn(z[j][i][k], minus2, __fadd2_rn(g[j][i][k], minus1)), by);
         if constexpr (!kJoin) {
-          if (c.dx) zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, to, i, column(i), width, edge, o);
+          if (c.dx) zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, slot, i, column(i), width, edge, o);
           continue;
         }
         if (third) {
@@ -160,11 +142,11 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
 #pragma unroll
           for (int k = 0; k < H; ++k) o[k] = __fadd2_rn(o[k], q[k]);
         }
-        if (c.dres) zp_write<T, kLying>(t, static_cast<char *>(c.dres) + at, to, i, column(i), width, edge, o);
+        if (c.dres) zp_write<T, kLying>(t, static_cast<char *>(c.dres) + at, slot, i, column(i), width, edge, o);
         if (!c.dx) continue;
 #pragma unroll
         for (int k = 0; k < H && drops; ++k) o[k] = kept.drop(o[k], i, k, limit, c.drop.scale);
-        zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, c.dres ? to + p.slot : to, i, column(i), width, edge, o);
+        zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, slot + p.slot, i, column(i), width, edge, o);
       }
     }
     if constexpr (kLying == kZpShifted) {
@@ -173,9 +155,9 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       for (int j = 0; j < R; ++j) {
         if (turn >= own.n[j]) continue;
         const int64_t at = out + j * next;
-        const uint32_t from = kHeld ? slots + j * row_slots : results;
+        const uint32_t from = slots + j * row_slots;
         if (kJoin && c.dres) zp_store_row<T, M>(t, static_cast<char *>(c.dres) + at, from, width);
-        if (c.dx) zp_store_row<T, M>(t, static_cast<char *>(c.dx) + at, kJoin && c.dres ? from + p.slot : from, width);
+        if (c.dx) zp_store_row<T, M>(t, static_cast<char *>(c.dx) + at, kJoin ? from + p.slot : from, width);
       }
       sx.advance();
       sy.advance();
@@ -186,7 +168,20 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     slots = slots + stage_bytes == ring + ring_bytes ? ring : slots + stage_bytes;
   }
   zp_copy_wait(2);
+  t.meet();                                    // (nobody writes to a block that has gone)
   if (!c.partial) return;
+  float *const part = c.partial + (size_t)t.block() * 2 * c.width;
+  if constexpr (kWide) {                       // each thread has columns that nobody else has
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        const int at = column(i) + 2 * k;
+        if ((unsigned)at < (unsigned)width) { part[at] = gw[i][k].x; part[c.width + at] = gb[i][k].x; }
+        if ((unsigned)(at + 1) < (unsigned)width) { part[at + 1] = gw[i][k].y; part[c.width + at + 1] = gb[i][k].y; }
+      }
+    return;
+  }
   // The teams' sums through shared memory, in order; of aligned rows those within a warp first, which have the same
   // columns (of cycled rows each class has its own)
   constexpr bool kByWarp = kLying != kZpCycled;
@@ -221,7 +216,6 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       }
   }
   __syncthreads();
-  float *const part = c.partial + (size_t)blockIdx.x * 2 * c.width;
   for (int i = threadIdx.x; i < 2 * width; i += kZpTeamThreads) {
     const int at = i < width ? i : row + (i - width);
     float sum = 0.f;
@@ -232,29 +226,31 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
 
 bool is_join(const ZpNormCall &c) { return c.dsum || c.dres || c.drop.state; }
 
-template <typename T, int kLying, bool kFull, int E, int R, bool kJoin>
-int launch(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+template <typename T, int kLying, bool kFull, int E, int R, bool kJoin, bool kWide>
+int launch(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   static ZpSmemOptIn opt_in;
-  if (int rc = zp_ensure_smem(norm_bwd_team_kernel<T, kLying, kFull, E, R, kJoin>, p.smem, opt_in)) return rc;
-  zp_launch(norm_bwd_team_kernel<T, kLying, kFull, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
-  ZP_LAUNCH_CHECK("norm_bwd_team_kernel");
-  return ZP_OK;
+  static ZpClusters clusters;
+  return zp_launch_teams<kWide>(norm_bwd_team_kernel<T, kLying, kFull, E, R, kJoin, kWide>, "norm_bwd_team_kernel", c, p,
+                                opt_in, clusters, st);
 }
 template <typename T, int kLying, bool kFull, bool kJoin>
-int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+int by_elements(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
+  if constexpr (kLying != kZpShifted) {
+    if (p.ranks > 1) return launch<T, kLying, kFull, 8, 2, kJoin, true>(c, p, st);    // rows of more than a block's elements
+  } else {
+    if (p.elements == 16) return launch<T, kLying, kFull, 16, 1, kJoin, false>(c, p, st);
+  }
   if constexpr (kLying != kZpShifted || !kJoin)
-    if (p.rows == 2) return launch<T, kLying, kFull, 8, 2, kJoin>(c, p, st);
-  if (p.elements == 8) return launch<T, kLying, kFull, 8, 1, kJoin>(c, p, st);
-  return p.elements == 16 ? launch<T, kLying, kFull, 16, 1, kJoin>(c, p, st)
-                          : launch<T, kLying, kFull, 32, 1, kJoin>(c, p, st);
+    if (p.rows == 2) return launch<T, kLying, kFull, 8, 2, kJoin, false>(c, p, st);
+  return launch<T, kLying, kFull, 8, 1, kJoin, false>(c, p, st);
 }
-template <typename T, bool kJoin> int by_lying(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+template <typename T, bool kJoin> int by_lying(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   if (p.full) return by_elements<T, kZpAligned, true, kJoin>(c, p, st);
   if (p.lying == kZpAligned) return by_elements<T, kZpAligned, false, kJoin>(c, p, st);
   return p.lying == kZpCycled ? by_elements<T, kZpCycled, false, kJoin>(c, p, st)
                               : by_elements<T, kZpShifted, false, kJoin>(c, p, st);
 }
-template <typename T> int by_kind(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+template <typename T> int by_kind(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   return is_join(c) ? by_lying<T, true>(c, p, st) : by_lying<T, false>(c, p, st);
 }
 
@@ -269,17 +265,16 @@ int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_
   // Two rows at a time, as in the forward: 16384 x 4096 bf16 93 us -> 76, joined 153 -> 132, 400000 x 32 23 -> 20.
   // Joined rows of a warp or less (60000 x 128 fp32 29 -> 31) or that are not aligned (30011 x 1001 fp16 150 -> 185:
   // registers) are better one by one.
-  const bool two = each >= 32 && (!join || (lying != kZpShifted && c.width > 256));
-  // (rows of many elements are read twice, so that their results cannot pass through the slots they came in)
-  const int results = lying != kZpShifted ? 0 : c.dx && c.dres ? 2 : 1;
+  const bool wide = lying != kZpShifted && c.width > 8 * kZpTeamThreads - 7;
+  const bool two = wide || (each >= 32 && (!join || (lying != kZpShifted && c.width > 256)));
   ZpTeamPlan p;
-  taken = c.dy && ((two && zp_team_plan(c, lying, arrays, 0, last, 8, 2, p)) ||
-                   zp_team_plan(c, lying, arrays, 0, last, 8, 1, p) ||
-                   zp_team_plan(c, lying, arrays, 0, last, 16, 1, p) ||
-                   zp_team_plan(c, lying, arrays, results, last, 32, 1, p));
+  taken = c.dy && ((two && zp_team_plan(c, lying, arrays, last, 8, 2, p)) ||
+                   (!wide && zp_team_plan(c, lying, arrays, last, 8, 1, p)) ||
+                   (!wide && lying == kZpShifted && zp_team_plan(c, lying, arrays, last, 16, 1, p)));
   if (!taken) return ZP_OK;
-  parts = (int)p.blocks;
-  if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);
-  if (c.dtype == ZP_F16) return by_kind<__half>(c, p, st);
-  return by_kind<__nv_bfloat16>(c, p, st);
+  const int rc = c.dtype == ZP_F32   ? by_kind<float>(c, p, st)
+                 : c.dtype == ZP_F16 ? by_kind<__half>(c, p, st)
+                                     : by_kind<__nv_bfloat16>(c, p, st);
+  parts = (int)p.blocks / p.ranks;
+  return rc;
 }

@@ -8,16 +8,15 @@
 namespace {
 
 // E elements of a thread in each of R rows at a time
-template <typename T, int kLying, bool kFull, int E, int R, bool kJoin>
+template <typename T, int kLying, bool kFull, int E, int R, bool kJoin, bool kWide>
 __global__ void __launch_bounds__(kZpTeamThreads, 1)
 norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant__ ZpTeamPlan p) {
   zp_after_previous();
   constexpr int V = kZpVec<T>, H = V / 2, M = E / V, A = kJoin ? 2 : 1;
-  constexpr bool kHeld = E <= 16;              // weight and bias stay in registers
   extern __shared__ __align__(16) char smem[];
-  const ZpTeam t(p.team, reinterpret_cast<float *>(smem));
+  const ZpTeam<kWide> t(p.team, p.ranks, reinterpret_cast<float *>(smem));
   const int width = (int)c.width, stages = p.stages;
-  char *const after_red = smem + sizeof(float) * 2 * 4 * kZpTeamWarps;
+  char *const after_red = smem + kZpSumsBytes;
   uint8_t *const bytes = reinterpret_cast<uint8_t *>(after_red) + t.index * p.bytes;
   const uint32_t stage_bytes = A * R * p.slot, ring_bytes = stages * stage_bytes;
   const uint32_t ring = zp_shared(after_red) + p.bytes * (kZpTeamThreads / p.team) + t.index * ring_bytes;
@@ -38,15 +37,15 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
 
   const bool wide = c.param_dtype == ZP_F32;
-  auto column = [&](int i) { return (t.lane + i * t.size) * V - own.before; };
+  auto column = [&](int i) { return t.piece(i) * V - own.before; };
   // whether the row has any of a thread's piece, and whether there may be a piece that it does not fill
   auto has = [&](int i) { return kFull || (column(i) < width && (kLying != kZpCycled || column(i) + V > 0)); };
   bool edge = false;
 #pragma unroll
   for (int i = 0; i < M && kLying != kZpAligned; ++i) edge = edge || (has(i) && (column(i) < 0 || column(i) + V > width));
-  float2 w[kHeld ? M : 1][H], b[kHeld ? M : 1][H];
+  float2 w[M][H], b[M][H];
 #pragma unroll
-  for (int i = 0; i < (kHeld ? M : 0); ++i) {
+  for (int i = 0; i < M; ++i) {
     zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, w[i]);
     zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, b[i]);
   }
@@ -61,6 +60,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   const float inv_w = 1.f / (float)width;
   const int64_t row_bytes = c.width * (int64_t)sizeof(T), next = own.next * row_bytes;
   int64_t out = own.first * row_bytes - own.before * (int)sizeof(T);        // of the rows that are worked on, in every result
+  t.meet();                                    // the team's blocks run
   uint32_t slots = ring, behind = ring + (stages - 1) * stage_bytes;
   for (int turn = 0; turn < own.turns; ++turn) {
     zp_copy_wait(stages);
@@ -136,18 +136,12 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
 #pragma unroll
       for (int i = 0; i < M; ++i) {
         if (turn >= own.n[j] || !has(i)) continue;
-        float2 ww[H], bb[H];
-        if constexpr (!kHeld) {
-          zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, ww);
-          zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, bb);
-        }
 #pragma unroll
         for (int k = 0; k < H; ++k)
-          v[j][i][k] = __ffma2_rn(__fmul2_rn(v[j][i][k], both), kHeld ? w[kHeld ? i : 0][k] : ww[k],
-                                  kHeld ? b[kHeld ? i : 0][k] : bb[k]);
+          v[j][i][k] = __ffma2_rn(__fmul2_rn(v[j][i][k], both), w[i][k], b[i][k]);
         zp_write<T, kLying>(t, y, slots + (j * A + A - 1) * p.slot, i, column(i), width, edge, v[j][i]);
       }
-      if (t.lane == 0 && c.mean && turn < own.n[j]) {
+      if (t.piece(0) == 0 && c.mean && turn < own.n[j]) {
         const int64_t r = own.first + turn * own.step + j * own.next;
         c.mean[r] = s[j];
         c.rstd[r] = rstd;
@@ -170,31 +164,33 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     slots = slots + stage_bytes == ring + ring_bytes ? ring : slots + stage_bytes;
   }
   zp_copy_wait(2);
+  t.meet();                                    // (nobody writes to a block that has gone)
 }
 
-template <typename T, int kLying, bool kFull, int E, int R, bool kJoin>
-int launch(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+template <typename T, int kLying, bool kFull, int E, int R, bool kJoin, bool kWide>
+int launch(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   static ZpSmemOptIn opt_in;
-  if (int rc = zp_ensure_smem(norm_fwd_team_kernel<T, kLying, kFull, E, R, kJoin>, p.smem, opt_in)) return rc;
-  zp_launch(norm_fwd_team_kernel<T, kLying, kFull, E, R, kJoin>, p.blocks, kZpTeamThreads, p.smem, st, c, p);
-  ZP_LAUNCH_CHECK("norm_fwd_team_kernel");
-  return ZP_OK;
+  static ZpClusters clusters;
+  return zp_launch_teams<kWide>(norm_fwd_team_kernel<T, kLying, kFull, E, R, kJoin, kWide>, "norm_fwd_team_kernel", c, p,
+                                opt_in, clusters, st);
 }
 template <typename T, int kLying, bool kFull, bool kJoin>
-int by_elements(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
-  if (p.elements == 8) return launch<T, kLying, kFull, 8, 1, kJoin>(c, p, st);
-  if (p.elements == 32) return launch<T, kLying, kFull, 32, 1, kJoin>(c, p, st);
+int by_elements(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
+  if (p.ranks > 1) {                           // rows of more than a block's elements
+    if constexpr (kLying != kZpShifted) return launch<T, kLying, kFull, 16, sizeof(T) == 2 ? 2 : 1, kJoin, true>(c, p, st);
+  }
+  if (p.elements == 8) return launch<T, kLying, kFull, 8, 1, kJoin, false>(c, p, st);
   if constexpr (sizeof(T) == 2)
-    if (p.rows == 2) return launch<T, kLying, kFull, 16, 2, kJoin>(c, p, st);
-  return launch<T, kLying, kFull, 16, 1, kJoin>(c, p, st);
+    if (p.rows == 2) return launch<T, kLying, kFull, 16, 2, kJoin, false>(c, p, st);
+  return launch<T, kLying, kFull, 16, 1, kJoin, false>(c, p, st);
 }
-template <typename T, bool kJoin> int by_lying(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+template <typename T, bool kJoin> int by_lying(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   if (p.full) return by_elements<T, kZpAligned, true, kJoin>(c, p, st);
   if (p.lying == kZpAligned) return by_elements<T, kZpAligned, false, kJoin>(c, p, st);
   return p.lying == kZpCycled ? by_elements<T, kZpCycled, false, kJoin>(c, p, st)
                               : by_elements<T, kZpShifted, false, kJoin>(c, p, st);
 }
-template <typename T> int by_kind(const ZpNormCall &c, const ZpTeamPlan &p, cudaStream_t st) {
+template <typename T> int by_kind(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   return c.res ? by_lying<T, true>(c, p, st) : by_lying<T, false>(c, p, st);
 }
 
@@ -208,12 +204,12 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
   // turns to share out (60000 x 128 bf16 9.5 -> 10.4).  Few elements are spread over more threads.
   const int64_t each = c.rows * c.width / ((int64_t)148 * kZpTeamThreads);       // elements a thread
   const int arrays = c.res ? 2 : 1;
-  const bool two = each >= 64 && c.width > 512 && size == 2 && (!c.res || c.drop.state);
+  const bool wide = c.width > 16 * kZpTeamThreads - 7;
+  const bool two = size == 2 && (wide || (each >= 64 && c.width > 512 && (!c.res || c.drop.state)));
   ZpTeamPlan p;
-  taken = (two && zp_team_plan(c, lying, arrays, 0, 0, 16, 2, p)) ||
-          (each >= 32 && zp_team_plan(c, lying, arrays, 0, 0, 16, 1, p)) ||
-          zp_team_plan(c, lying, arrays, 0, 0, 8, 1, p) || zp_team_plan(c, lying, arrays, 0, 0, 16, 1, p) ||
-          zp_team_plan(c, lying, arrays, 0, 0, 32, 1, p);
+  taken = (two && zp_team_plan(c, lying, arrays, 0, 16, 2, p)) ||
+          ((wide || each >= 32 || c.width > 8 * kZpTeamThreads - 7) && zp_team_plan(c, lying, arrays, 0, 16, 1, p)) ||
+          (!wide && zp_team_plan(c, lying, arrays, 0, 8, 1, p) && p.ranks == 1);
   if (!taken) return ZP_OK;
   if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);
   if (c.dtype == ZP_F16) return by_kind<__half>(c, p, st);
