@@ -63,7 +63,7 @@ __device__ __forceinline__ void kept_words(const ZpPhiloxKey<true> &key, int64_t
 
 template <typename T, int kHow>
 __global__ void __launch_bounds__(kThreads, 4)
-dropout_pieces_kernel(int64_t pieces, int64_t per_row, int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx,
+dropout_pieces_kernel(int64_t pieces, int rest, int64_t per_row, int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx,
                       ZpDrop drop, T *__restrict__ y, int64_t ldy) {
   zp_after_previous();
   constexpr int kAhead = 4, V = kZpVec<T>;
@@ -72,6 +72,11 @@ dropout_pieces_kernel(int64_t pieces, int64_t per_row, int64_t rows, int64_t wid
   const int lane = threadIdx.x % 32;
   const int64_t step = (int64_t)gridDim.x * kThreads * kAhead;
   const bool small = rows * width <= 0xffffffffll;
+  if (blockIdx.x == 0 && threadIdx.x < rest) {                                 // behind the last whole counter
+    const int64_t e = pieces * V + threadIdx.x, r = e / width;
+    const uint32_t kept = zp_philox_kept(key, e / 8, limit) >> threadIdx.x & 1;
+    y[e] = zp_rounded<T>(kept ? zp_float(x[r * ldx + e - r * width]) * drop.scale : 0.f);
+  }
   for (int64_t p0 = (int64_t)(blockIdx.x * kThreads + threadIdx.x - lane) * kAhead; p0 < pieces; p0 += step) {
     uint4 in[kAhead];
     T *to[kHow == kRows ? kAhead : 1];
@@ -96,11 +101,16 @@ dropout_pieces_kernel(int64_t pieces, int64_t per_row, int64_t rows, int64_t wid
         }
       }
     } else {
+      const int64_t e = (p0 + lane) * V;
+      int64_t r = small ? (uint32_t)e / (uint32_t)width : e / width, c = e - r * width;      // row, column of a piece
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int64_t e = (p0 + 32 * i + lane) * V;
+      for (int i = 0; i < kAhead; ++i, c += 32 * V) {
+        if (c >= width) {
+          const int64_t more = width >= 32 * V ? 1 : c / width;
+          r += more;
+          c -= more * width;
+        }
         if (32 * i >= left) continue;
-        const int64_t r = small ? (uint32_t)e / (uint32_t)width : e / width, c = e - r * width;
         const char *const at = reinterpret_cast<const char *>(x + r * ldx + c);
         const int place = (int)(reinterpret_cast<uintptr_t>(at) & 15);
         const char *const from = at - place;
@@ -137,18 +147,18 @@ dropout_pieces_kernel(int64_t pieces, int64_t per_row, int64_t rows, int64_t wid
   }
 }
 
-// Elements first .. rows * width - 1 wherever they lie: the last ones of a call, and results that are not row
-// behind row.  A warp goes through 256 of them, works out the 32 counters and hands each lane its bits.
+// Elements wherever they lie, for results that are not row behind row or are fewer than eight.  A warp goes
+// through 256 of them, works out the 32 counters and hands each lane its bits.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-dropout_elements_kernel(int64_t first, int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, ZpDrop drop,
+dropout_elements_kernel(int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx, ZpDrop drop,
                         T *__restrict__ y, int64_t ldy) {
   zp_after_previous();
   const ZpPhiloxKey<true> key = zp_philox_key<true>(drop.state);
   const uint32_t limit = zp_drop_limit(drop.threshold);
   const int lane = threadIdx.x % 32;
   const int64_t n = rows * width, step = (int64_t)gridDim.x * kThreads * 8;
-  for (int64_t e0 = first + (int64_t)(blockIdx.x * kThreads + threadIdx.x - lane) * 8; e0 < n; e0 += step) {
+  for (int64_t e0 = (int64_t)(blockIdx.x * kThreads + threadIdx.x - lane) * 8; e0 < n; e0 += step) {
     const uint32_t mine = zp_philox_kept(key, e0 / 8 + lane, limit);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -320,24 +330,23 @@ template <typename T> int run_dropout(int64_t rows, int64_t width, const void *x
   }
   const bool whole = !misplaced(x, 16) && !misplaced(y, 16) &&
                      (rows == 1 || (width % 8 == 0 && ldx % V == 0 && ldy % V == 0));
-  int64_t first = 0;                                          // elements that go by pieces, whole counters of them
   if (whole || (behind && !misplaced(y, 16))) {
-    first = rows * width / 8 * 8;
+    const int64_t first = rows * width / 8 * 8;              // elements that go by pieces, whole counters of them
     const int64_t pieces = first / V;
     const unsigned blocks = blocks_for(zp_ceil_div(pieces, 4 * kThreads), 148 * 8);
     if (pieces > 0) {
       const auto kernel = !whole      ? dropout_pieces_kernel<T, kGather>
                           : rows == 1 ? dropout_pieces_kernel<T, kFlat>
                                       : dropout_pieces_kernel<T, kRows>;
-      zp_launch(kernel, blocks, kThreads, 0, st, pieces, width / V, rows, width, in, ldx, drop, out, ldy);
+      const int rest = (int)(rows * width - first);          // (none where rows are whole counters)
+      zp_launch(kernel, blocks, kThreads, 0, st, pieces, rest, width / V, rows, width, in, ldx, drop, out, ldy);
       ZP_LAUNCH_CHECK("dropout_pieces_kernel");
+      return ZP_OK;
     }
   }
-  if (first < rows * width) {
-    zp_launch(dropout_elements_kernel<T>, blocks_for(zp_ceil_div(rows * width - first, 8 * kThreads), 148 * 8), kThreads,
-              0, st, first, rows, width, in, ldx, drop, out, ldy);
-    ZP_LAUNCH_CHECK("dropout_elements_kernel");
-  }
+  zp_launch(dropout_elements_kernel<T>, blocks_for(zp_ceil_div(rows * width, 8 * kThreads), 148 * 8), kThreads, 0, st,
+            rows, width, in, ldx, drop, out, ldy);
+  ZP_LAUNCH_CHECK("dropout_elements_kernel");
   return ZP_OK;
 }
 

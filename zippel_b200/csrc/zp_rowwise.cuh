@@ -569,12 +569,14 @@ inline int64_t zp_whole_cycles(const ZpTeamPlan &p, int64_t most) {
   const int64_t by = p.cycle > teams ? p.cycle / teams : 1;
   return most / by * by;
 }
+// Elements of a row's pieces
+inline int64_t zp_span(const ZpNormCall &c, int lying) { return lying == kZpCycled ? c.width + 7 : c.width; }
 // `arrays` come in per row; `last_per_element`: bytes of shared memory per element of a block's teams that
 // the kernel needs when the ring is done with.  False: this does not fit.
 inline bool zp_team_plan(const ZpNormCall &c, int lying, int arrays, size_t last_per_element, int elements, int rows,
                          ZpTeamPlan &p) {
   const int64_t size = c.dtype == ZP_F32 ? 4 : 2;
-  const int64_t span = lying == kZpCycled ? c.width + 7 : c.width;             // elements of a row's pieces
+  const int64_t span = zp_span(c, lying);
   p.ranks = 1;
   while (span > (int64_t)kZpTeamThreads * elements * p.ranks && p.ranks <= kZpMostRanks) p.ranks *= 2;
   // (pieces of a shifted row that lie in two blocks would have to be put together across them)

@@ -237,9 +237,9 @@ template <typename T, int kLying, bool kFull, bool kJoin>
 int by_elements(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   if constexpr (kLying != kZpShifted) {
     if (p.ranks > 1) return launch<T, kLying, kFull, 8, 2, kJoin, true>(c, p, st);    // rows of more than a block's elements
-  } else {
-    if (p.elements == 16) return launch<T, kLying, kFull, 16, 1, kJoin, false>(c, p, st);
   }
+  if constexpr (kLying == kZpShifted || (sizeof(T) == 2 && !kJoin))
+    if (p.elements == 16) return launch<T, kLying, kFull, 16, 1, kJoin, false>(c, p, st);
   if constexpr (kLying != kZpShifted || !kJoin)
     if (p.rows == 2) return launch<T, kLying, kFull, 8, 2, kJoin, false>(c, p, st);
   return launch<T, kLying, kFull, 8, 1, kJoin, false>(c, p, st);
@@ -265,12 +265,15 @@ int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_
   // Two rows at a time, as in the forward: 16384 x 4096 bf16 93 us -> 76, joined 153 -> 132, 400000 x 32 23 -> 20.
   // Joined rows of a warp or less (60000 x 128 fp32 29 -> 31) or that are not aligned (30011 x 1001 fp16 150 -> 185:
   // registers) are better one by one.
-  const bool wide = lying != kZpShifted && c.width > 8 * kZpTeamThreads - 7;
-  const bool two = wide || (each >= 32 && (!join || (lying != kZpShifted && c.width > 256)));
+  const bool two = each >= 32 && (!join || (lying != kZpShifted && c.width > 256));
+  // Rows of more than 4096 elements: sixteen to a thread where that leaves registers enough (8192 x 8192 bf16 92 us, by
+  // clusters 121), else a cluster a row (2048 x 8192 fp32 joined 76 us, sixteen to a thread 88).
+  const bool over = zp_span(c, lying) > 8 * kZpTeamThreads;
+  const bool many = over && (lying == kZpShifted || (c.dtype != ZP_F32 && !join)), wide = over && lying != kZpShifted;
   ZpTeamPlan p;
-  taken = c.dy && ((two && zp_team_plan(c, lying, arrays, last, 8, 2, p)) ||
-                   (!wide && zp_team_plan(c, lying, arrays, last, 8, 1, p)) ||
-                   (!wide && lying == kZpShifted && zp_team_plan(c, lying, arrays, last, 16, 1, p)));
+  taken = c.dy && ((many && zp_team_plan(c, lying, arrays, last, 16, 1, p) && p.ranks == 1) ||
+                   ((two || wide) && zp_team_plan(c, lying, arrays, last, 8, 2, p)) ||
+                   (!wide && zp_team_plan(c, lying, arrays, last, 8, 1, p)));
   if (!taken) return ZP_OK;
   const int rc = c.dtype == ZP_F32   ? by_kind<float>(c, p, st)
                  : c.dtype == ZP_F16 ? by_kind<__half>(c, p, st)

@@ -204,11 +204,12 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
   // turns to share out (60000 x 128 bf16 9.5 -> 10.4).  Few elements are spread over more threads.
   const int64_t each = c.rows * c.width / ((int64_t)148 * kZpTeamThreads);       // elements a thread
   const int arrays = c.res ? 2 : 1;
-  const bool wide = c.width > 16 * kZpTeamThreads - 7;
+  const int64_t span = zp_span(c, lying);
+  const bool wide = span > 16 * kZpTeamThreads;
   const bool two = size == 2 && (wide || (each >= 64 && c.width > 512 && (!c.res || c.drop.state)));
   ZpTeamPlan p;
   taken = (two && zp_team_plan(c, lying, arrays, 0, 16, 2, p)) ||
-          ((wide || each >= 32 || c.width > 8 * kZpTeamThreads - 7) && zp_team_plan(c, lying, arrays, 0, 16, 1, p)) ||
+          ((wide || each >= 32 || span > 8 * kZpTeamThreads) && zp_team_plan(c, lying, arrays, 0, 16, 1, p)) ||
           (!wide && zp_team_plan(c, lying, arrays, 0, 8, 1, p) && p.ranks == 1);
   if (!taken) return ZP_OK;
   if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);
