@@ -238,7 +238,7 @@ int by_elements(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   if constexpr (kLying != kZpShifted) {
     if (p.ranks > 1) return launch<T, kLying, kFull, 8, 2, kJoin, true>(c, p, st);    // rows of more than a block's elements
   }
-  if constexpr (kLying == kZpShifted || (sizeof(T) == 2 && !kJoin))
+  if constexpr (kLying == kZpShifted || (sizeof(T) == 2))
     if (p.elements == 16) return launch<T, kLying, kFull, 16, 1, kJoin, false>(c, p, st);
   if constexpr (kLying != kZpShifted || !kJoin)
     if (p.rows == 2) return launch<T, kLying, kFull, 8, 2, kJoin, false>(c, p, st);
@@ -266,10 +266,10 @@ int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_
   // Joined rows of a warp or less (60000 x 128 fp32 29 -> 31) or that are not aligned (30011 x 1001 fp16 150 -> 185:
   // registers) are better one by one.
   const bool two = each >= 32 && (!join || (lying != kZpShifted && c.width > 256));
-  // Rows of more than 4096 elements: sixteen to a thread where that leaves registers enough (8192 x 8192 bf16 92 us, by
-  // clusters 121), else a cluster a row (2048 x 8192 fp32 joined 76 us, sixteen to a thread 88).
+  // Rows of more than 4096 elements: sixteen to a thread up to 8192 in 16 bits (8192 x 8192 bf16 91 us, by clusters 121;
+  // joined 160, 196), else a cluster a row (2048 x 8192 fp32 joined 76 us, sixteen to a thread 88).
   const bool over = zp_span(c, lying) > 8 * kZpTeamThreads;
-  const bool many = over && (lying == kZpShifted || (c.dtype != ZP_F32 && !join)), wide = over && lying != kZpShifted;
+  const bool many = over && (lying == kZpShifted || c.dtype != ZP_F32), wide = over && lying != kZpShifted;
   ZpTeamPlan p;
   taken = c.dy && ((many && zp_team_plan(c, lying, arrays, last, 16, 1, p) && p.ranks == 1) ||
                    ((two || wide) && zp_team_plan(c, lying, arrays, last, 8, 2, p)) ||

@@ -43,9 +43,10 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   bool edge = false;
 #pragma unroll
   for (int i = 0; i < M && kLying != kZpAligned; ++i) edge = edge || (has(i) && (column(i) < 0 || column(i) + V > width));
-  float2 w[M][H], b[M][H];
+  constexpr bool kHeld = E <= 16;              // weight and bias stay in registers
+  float2 w[kHeld ? M : 1][H], b[kHeld ? M : 1][H];
 #pragma unroll
-  for (int i = 0; i < M; ++i) {
+  for (int i = 0; i < (kHeld ? M : 0); ++i) {
     zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, w[i]);
     zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, b[i]);
   }
@@ -136,9 +137,13 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
 #pragma unroll
       for (int i = 0; i < M; ++i) {
         if (turn >= own.n[j] || !has(i)) continue;
+        float2 (&ww)[H] = w[kHeld ? i : 0], (&bb)[H] = b[kHeld ? i : 0];
+        if constexpr (!kHeld) {
+          zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, ww);
+          zp_params<T>(c.b, wide, p.vectors, column(i), width, 0.f, bb);
+        }
 #pragma unroll
-        for (int k = 0; k < H; ++k)
-          v[j][i][k] = __ffma2_rn(__fmul2_rn(v[j][i][k], both), w[i][k], b[i][k]);
+        for (int k = 0; k < H; ++k) v[j][i][k] = __ffma2_rn(__fmul2_rn(v[j][i][k], both), ww[k], bb[k]);
         zp_write<T, kLying>(t, y, slots + (j * A + A - 1) * p.slot, i, column(i), width, edge, v[j][i]);
       }
       if (t.piece(0) == 0 && c.mean && turn < own.n[j]) {
@@ -179,6 +184,8 @@ int by_elements(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   if (p.ranks > 1) {                           // rows of more than a block's elements
     if constexpr (kLying != kZpShifted) return launch<T, kLying, kFull, 16, sizeof(T) == 2 ? 2 : 1, kJoin, true>(c, p, st);
   }
+  if constexpr (kLying == kZpAligned)
+    if (p.elements == 32) return launch<T, kLying, kFull, 32, 1, kJoin, false>(c, p, st);
   if (p.elements == 8) return launch<T, kLying, kFull, 8, 1, kJoin, false>(c, p, st);
   if constexpr (sizeof(T) == 2)
     if (p.rows == 2) return launch<T, kLying, kFull, 16, 2, kJoin, false>(c, p, st);
@@ -207,8 +214,11 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
   const int64_t span = zp_span(c, lying);
   const bool wide = span > 16 * kZpTeamThreads;
   const bool two = size == 2 && (wide || (each >= 64 && c.width > 512 && (!c.res || c.drop.state)));
+  // Rows of more than 8192 elements: a cluster a row, which waits for its blocks' sums, or up to 16384, aligned and
+  // where the ring has room for them, 32 elements to a thread (4096 x 16384 bf16 79 us, by clusters 94)
   ZpTeamPlan p;
-  taken = (two && zp_team_plan(c, lying, arrays, 0, 16, 2, p)) ||
+  taken = (wide && lying == kZpAligned && zp_team_plan(c, lying, arrays, 0, 32, 1, p) && p.ranks == 1) ||
+          (two && zp_team_plan(c, lying, arrays, 0, 16, 2, p)) ||
           ((wide || each >= 32 || span > 8 * kZpTeamThreads) && zp_team_plan(c, lying, arrays, 0, 16, 1, p)) ||
           (!wide && zp_team_plan(c, lying, arrays, 0, 8, 1, p) && p.ranks == 1);
   if (!taken) return ZP_OK;
