@@ -202,40 +202,37 @@ template <bool kWide> struct ZpTeam {
     }
     const int at = threadIdx.x & 31;
     constexpr int kOwn = 32 / K;               // lanes that add up one value
-    float s;
-    if constexpr (K == 4) {
-      const bool hi = at & 16, up = at & 8;
-      const float a = (hi ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 16);
-      const float b = (hi ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 16);
-      s = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 8);
-    } else if constexpr (K == 2) {
-      const bool hi = at & 16;
-      s = (hi ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[1], 16);
-    } else {
-      s = v[0];
-    }
+    float s[K];
 #pragma unroll
-    for (int o = kOwn / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int k = 0; k < K; ++k) s[k] = v[k];
+#pragma unroll
+    for (int left = K / 2, o = 16; left > 0; left /= 2, o /= 2) {
+      const bool up = at & o;
+#pragma unroll
+      for (int k = 0; k < left; ++k)
+        s[k] = (up ? s[k + left] : s[k]) + __shfl_xor_sync(0xffffffffu, up ? s[k] : s[k + left], o);
+    }
+    float one = s[0];                          // of value at / kOwn
+#pragma unroll
+    for (int o = kOwn / 2; o > 0; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
     if (size > 32) {
       float *const buf = red + (turn & 1) * (kZpTeamWarps * 4);
-      if (at % kOwn == 0) buf[(threadIdx.x >> 5) * K + at / kOwn] = s;
+      if (at % kOwn == 0) buf[(threadIdx.x >> 5) * K + at / kOwn] = one;
       sync();
       const int n = size >> 5, first = index * n;            // warps of the team
       const float *from = buf + at / kOwn;
-      s = from[(first + (at % kOwn & (n - 1))) * K];
-      if (kOwn == 8 && n == 16) s += from[(first + at % kOwn + 8) * K];
+      one = from[(first + (at % kOwn & (n - 1))) * K];
+#pragma unroll
+      for (int w = kOwn; w < kZpTeamWarps; w += kOwn)
+        if (w < n) one += from[(first + at % kOwn + w) * K];
 #pragma unroll
       for (int o = kOwn / 2; o > 0; o >>= 1)
-        if (o < n) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (o < n) one += __shfl_xor_sync(0xffffffffu, one, o);
     } else if (order) {
       __syncwarp();
     }
-    if constexpr (K == 1) {
-      v[0] = s;
-    } else {
 #pragma unroll
-      for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, s, k * kOwn);
-    }
+    for (int k = 0; k < K; ++k) v[k] = K == 1 ? one : __shfl_sync(0xffffffffu, one, k * kOwn);
     if constexpr (kWide) {                     // the blocks' sums, added by each in the same order
       float *const buf = red + 2 * 4 * kZpTeamWarps + (turn & 1) * (kZpMostRanks * 4);
       if (lane < ranks * K) {
