@@ -367,6 +367,21 @@ def test_element_numbers_past_32_bits():
     del y
 
 
+def test_rows_past_32_bits():
+    """More than 2^32 elements (8.6 GB an array): rows on either side of the border, forward and backward."""
+    rows, width = 2 ** 20 + 64, 4096
+    g = torch.Generator("cuda").manual_seed(3)
+    x = torch.empty(rows, width, device="cuda", dtype=BF16).normal_(generator=g).requires_grad_()
+    gy = torch.empty(rows, width, device="cuda", dtype=BF16).normal_(generator=g)
+    y = rowwise().layer_norm(x, None, None, EPS)
+    gx, = torch.autograd.grad(y, x, gy)
+    for first in (0, 2 ** 19 - 4, 2 ** 20 - 4, rows - 8):
+        part = slice(first, first + 8)
+        want = Want(x.detach()[part].cpu(), None, None, gy[part].cpu(), BF16, BF16)
+        near(y[part], want.y, want.ty)
+        near(gx[part], want.gx, want.tgx)
+
+
 @pytest.mark.parametrize("dtype,width", [(F32, 128), (F32, 33), (BF16, 4096), (BF16, 520), (F16, 1001), (F16, 7),
                                          (BF16, 16384), (F32, 20011)])
 @pytest.mark.parametrize("p", [0.0, 0.25, 1.0])

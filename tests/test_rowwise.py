@@ -93,12 +93,16 @@ def test_refusals_of_the_c_abi(lib):
     assert addb(p=-0.5) == 1 and addb(st=None) == 1 and addb(work=None) == 1
 
 
-def test_refusals_of_the_python_layer():
+def test_refusals_of_the_python_layer(lib):
     from zippel_b200.blocks import rowwise
     x = torch.zeros(2, 8)
     for call in (lambda: rowwise.layer_norm(x), lambda: rowwise.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64)),
                  lambda: rowwise.dropout_add_layer_norm(x, x)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+    with pytest.raises(TypeError):
+        rowwise.layer_norm([1.0, 2.0])
+    with pytest.raises(TypeError):
+        rowwise.dropout(x, "half", torch.zeros(2, dtype=torch.int64))
     with pytest.raises(ValueError):
         rowwise.ResidualNorm([torch.nn.Linear(8, 8)], 8, p=1.5)

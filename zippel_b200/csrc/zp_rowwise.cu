@@ -31,7 +31,8 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 
 // Dropout.  Each thread writes pieces of 16 bytes, kAhead of them 32 apart, whose loads are on the way together.
 // Bound by memory, with the generator close behind: of some 60 integer instructions for eight elements 20
-// are wide products.  In fp32 a piece is half of a counter's elements: of two neighbouring lanes each works
+// are wide products.  B200 (share of 6 450 GB/s): 16384 x 8192 bf16 87 to 90 us (0.93 to 0.96), 60000 x 128 fp32 11.0
+// (0.86), 20011 x 1023 fp16 14.8 (0.86) and, 1030 apart, 30.8 (0.41: each piece from two, and where it lies).  In fp32 a piece is half of a counter's elements: of two neighbouring lanes each works
 // out the counter of one of two pieces, and they swap words.
 //   kFlat    one row of aligned pieces from end to end
 //   kRows    `per_row` aligned pieces a row

@@ -1,11 +1,11 @@
 // Operators over the rows of a matrix: what their kernels share.
 //
-// A row is worked on by a team of 2 to 512 threads, or of a cluster of blocks of 512, E elements to a thread in
-// pieces of 16 bytes; a team
-// takes R rows at a time, so that what a row costs beside its elements (the joining of sums, barriers,
-// addresses) is shared.  Teams of a warp or less add up by shuffles, larger ones through shared memory and a
-// named barrier of their own.  Arithmetic on the elements goes by pairs (one instruction for two): these
-// kernels have 20 to 30 instruction slots for an element at the memory's speed, and spend 8 to 15.
+// A row is worked on by a team of 2 to 512 threads, or by a cluster of blocks of 512, E elements to a thread in
+// pieces of 16 bytes; a team takes R rows at a time, so that what a row costs beside its elements (the joining of
+// sums, barriers, addresses) is shared.  Teams of a warp or less add up by shuffles, larger ones through shared
+// memory and a named barrier of their own, clusters through each other's shared memory.  Arithmetic on the elements goes by pairs (one instruction for two): these
+// kernels have 20 to 35 instruction slots for an element at the memory's speed, and spend 11 to 20, or 28 to 41 with
+// dropout.
 //
 // Rows come in through a ring in shared memory that asynchronous copies keep filled: the 6.5 TB/s of the
 // memory want some 40 KB in flight on every SM, which registers do not hold beside the sums.

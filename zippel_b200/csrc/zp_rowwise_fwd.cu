@@ -3,6 +3,12 @@
 // Memory bound: a row is read once and the results are written once.  Mean and variance take two passes
 // over the row in registers, the variance from differences to the mean: sums of squares would lose a mean
 // that is large against the spread.
+//
+// B200, one kernel (share of 6 450 GB/s): 8192 x 4096 fp32 43 us (0.97), 16384 x 4096 bf16 48 (0.87; 11.3
+// instructions an element, 46 % of the issue slots: the waits of sixteen warps for each other's sums are what is
+// left), joined with dropout 96 (0.86; 28 instructions, half of them the generator), 60000 x 128 fp32 11.9 (0.80, of it two
+// for the launch and a turn that not every warp has), 30011 x 1001 fp16 40 (0.46: the ends of the rows are the
+// work of two lanes while the others wait).
 #include "zp_rowwise.cuh"
 
 namespace {
@@ -187,7 +193,7 @@ int by_elements(const ZpNormCall &c, ZpTeamPlan &p, cudaStream_t st) {
   if constexpr (kLying == kZpAligned)
     if (p.elements == 32) return launch<T, kLying, kFull, 32, 1, kJoin, false>(c, p, st);
   if (p.elements == 8) return launch<T, kLying, kFull, 8, 1, kJoin, false>(c, p, st);
-  if constexpr (sizeof(T) == 2)
+  if constexpr (sizeof(T) == 2 && (!kJoin || kLying == kZpAligned))
     if (p.rows == 2) return launch<T, kLying, kFull, 16, 2, kJoin, false>(c, p, st);
   return launch<T, kLying, kFull, 16, 1, kJoin, false>(c, p, st);
 }
@@ -207,13 +213,15 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
   const size_t size = c.dtype == ZP_F32 ? 4 : 2;
   const int lying = zp_lying(c, {{c.x, c.ldx}, {c.y, c.width}, {c.res, c.ldr}, {c.sum, c.width}});
   // Two rows at a time halve what joining the sums of a team of several warps costs (16384 x 4096 bf16 59 us ->
-  // 49), and leave the ring fewer stages (fp32 42 -> 50, joined without dropout 92 -> 99) and the blocks fewer
-  // turns to share out (60000 x 128 bf16 9.5 -> 10.4).  Few elements are spread over more threads.
+  // 49), and leave the ring fewer stages (fp32 42 -> 50, joined without dropout 92 -> 99), the blocks fewer
+  // turns to share out (60000 x 128 bf16 9.5 -> 10.4) and joined rows that are not aligned too few registers (30011 x
+  // 1001 fp16 72 -> 92).  Few elements are spread over more threads.
   const int64_t each = c.rows * c.width / ((int64_t)148 * kZpTeamThreads);       // elements a thread
   const int arrays = c.res ? 2 : 1;
   const int64_t span = zp_span(c, lying);
   const bool wide = span > 16 * kZpTeamThreads;
-  const bool two = size == 2 && (wide || (each >= 64 && c.width > 512 && (!c.res || c.drop.state)));
+  const bool two = size == 2 &&
+                   (wide || (each >= 64 && c.width > 512 && (!c.res || (c.drop.state && lying == kZpAligned))));
   // Rows of more than 8192 elements: a cluster a row, which waits for its blocks' sums, or up to 16384, aligned and
   // where the ring has room for them, 32 elements to a thread (4096 x 16384 bf16 79 us, by clusters 94)
   ZpTeamPlan p;
