@@ -510,3 +510,70 @@ def test_inputs_changed_before_the_backward_are_noticed():
     with pytest.raises(RuntimeError):          # first order only
         g, = torch.autograd.grad(rw.layer_norm(leaf, w, b), leaf, gy, create_graph=True)
         torch.autograd.grad(g.sum(), leaf)
+
+
+def test_nothing_dropped_through_the_c_abi_copies():
+    from zippel_b200 import _lib
+    state = torch.tensor([5, 6], device="cuda")
+    x = torch.randn(5, 12, device="cuda")
+    for width, ldy in ((12, 12), (12, 20), (7, 7)):
+        y = torch.full((5, ldy), -7.0, device="cuda")
+        _lib.run(x.device, "zp_dropout", 5, width, 0, x.data_ptr(), 12, 0.0, state.data_ptr(), y.data_ptr(), ldy)
+        assert torch.equal(y[:, :width], x[:, :width]) and bool((y[:, width:] == -7).all())
+
+
+def test_calls_that_torch_wraps():
+    """Tangents and batched tensors are refused, not read past; inference tensors and gradients of the same
+    tensor given twice are served."""
+    import torch.autograd.forward_ad as fwd
+    rw = rowwise()
+    x, w, b, gy, _ = up(*norm_case(8, 32, F32, F32, 8))
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        rw.layer_norm(fwd.make_dual(x, gy), w, b)
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda v: rw.layer_norm(v, w, b))(x.view(2, 4, 32))
+    with torch.inference_mode():
+        y = rw.layer_norm(x, w, b)
+        z, s = rw.dropout_add_layer_norm(x, x, w, b, 0.5, rw.dropout_state("cuda"))
+    assert torch.equal(y, rw.layer_norm(x, w, b)) and not y.requires_grad and z.shape == s.shape
+    leaf = x.clone().requires_grad_()
+    y, s = rw.dropout_add_layer_norm(leaf, leaf, w, b)
+    twice, = torch.autograd.grad(y, leaf, gy)
+    pair = [x.clone().requires_grad_() for _ in range(2)]
+    one, other = torch.autograd.grad(rw.dropout_add_layer_norm(*pair, w, b)[0], pair, gy)
+    assert torch.equal(twice, one + other)
+
+
+def test_two_streams_and_threads_at_once():
+    """The same leaves through forward and backward on two streams from two threads, many times: no scratch is
+    shared."""
+    import threading
+    rw = rowwise()
+    cases = [up(*norm_case(300, width, F32, F32, width)) for width in (1001, 4096)]
+    state = torch.tensor([1, 2], device="cuda")
+
+    def work(case):
+        x, w, b, gy, gs = case
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y, s = rw.dropout_add_layer_norm(leaves[0], gs, leaves[1], leaves[2], 0.3, state)
+        return [y.detach(), s.detach(), *torch.autograd.grad([y, s], leaves, [gy, gs])]
+
+    want = [work(c) for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                got = work(cases[i])
+                stream.synchronize()
+                if not all(torch.equal(a, c) for a, c in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1, 0)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -32,8 +32,9 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 // Dropout.  Each thread writes pieces of 16 bytes, kAhead of them 32 apart, whose loads are on the way together.
 // Bound by memory, with the generator close behind: of some 60 integer instructions for eight elements 20
 // are wide products.  B200 (share of 6 450 GB/s): 16384 x 8192 bf16 87 to 90 us (0.93 to 0.96), 60000 x 128 fp32 11.0
-// (0.86), 20011 x 1023 fp16 14.8 (0.86) and, 1030 apart, 30.8 (0.41: each piece from two, and where it lies).  In fp32 a piece is half of a counter's elements: of two neighbouring lanes each works
-// out the counter of one of two pieces, and they swap words.
+// (0.86), 20011 x 1023 fp16 14.8 (0.86) and, 1030 apart, 30.8 (0.41: each piece from two, and where it lies).
+// In fp32 a piece is half of a counter's elements: of two neighbouring lanes each works out the counter of one of
+// two pieces, and they swap words.
 //   kFlat    one row of aligned pieces from end to end
 //   kRows    `per_row` aligned pieces a row
 //   kGather  y lies row behind row; a piece of x is put together from the two that it lies in, at the end of
@@ -64,8 +65,8 @@ __device__ __forceinline__ void kept_words(const ZpPhiloxKey<true> &key, int64_t
 
 template <typename T, int kHow>
 __global__ void __launch_bounds__(kThreads, 4)
-dropout_pieces_kernel(int64_t pieces, int rest, int64_t per_row, int64_t rows, int64_t width, const T *__restrict__ x, int64_t ldx,
-                      ZpDrop drop, T *__restrict__ y, int64_t ldy) {
+dropout_pieces_kernel(int64_t pieces, int rest, int64_t per_row, int64_t rows, int64_t width,
+                      const T *__restrict__ x, int64_t ldx, ZpDrop drop, T *__restrict__ y, int64_t ldy) {
   zp_after_previous();
   constexpr int kAhead = 4, V = kZpVec<T>;
   const ZpPhiloxKey<true> key = zp_philox_key<true>(drop.state);
@@ -397,8 +398,17 @@ template <typename T, typename P> int run_bwd(const ZpNormCall &c, cudaStream_t 
                                    : CALL<__nv_bfloat16, __nv_bfloat16>(c, st);     \
   }
 
-int norm_fwd(ZpNormCall &c, int dtype, int param_dtype, cudaStream_t st) { c.dtype = dtype; c.param_dtype = param_dtype; BY_TYPES(run_fwd) }
-int norm_bwd(ZpNormCall &c, int dtype, int param_dtype, void *work, cudaStream_t st) { c.dtype = dtype; c.param_dtype = param_dtype; c.partial = c.dw || c.db ? static_cast<float *>(work) : nullptr; BY_TYPES(run_bwd) }
+int norm_fwd(ZpNormCall &c, int dtype, int param_dtype, cudaStream_t st) {
+  c.dtype = dtype;
+  c.param_dtype = param_dtype;
+  BY_TYPES(run_fwd)
+}
+int norm_bwd(ZpNormCall &c, int dtype, int param_dtype, void *work, cudaStream_t st) {
+  c.dtype = dtype;
+  c.param_dtype = param_dtype;
+  c.partial = c.dw || c.db ? static_cast<float *>(work) : nullptr;
+  BY_TYPES(run_bwd)
+}
 #undef BY_TYPES
 
 bool bad_param_type(int dtype, int param_dtype) { return param_dtype != dtype && param_dtype != ZP_F32; }
@@ -447,7 +457,10 @@ int zp_dropout(int64_t rows, int64_t width, int dtype, const void *x, int64_t ld
   cudaStream_t st = (cudaStream_t)stream;
   const size_t size = type_bytes(dtype);
   if (!drop.state) {                           // nothing is dropped
-    ZP_CUDA(cudaMemcpy2DAsync(y, ldy * size, x, ldx * size, width * size, rows, cudaMemcpyDeviceToDevice, st));
+    if ((ldx == width && ldy == width) || rows == 1)
+      ZP_CUDA(cudaMemcpyAsync(y, x, rows * width * size, cudaMemcpyDeviceToDevice, st));
+    else
+      ZP_CUDA(cudaMemcpy2DAsync(y, ldy * size, x, ldx * size, width * size, rows, cudaMemcpyDeviceToDevice, st));
     return ZP_OK;
   }
   if (dtype == ZP_F32) return run_dropout<float>(rows, width, x, ldx, drop, y, ldy, st);
