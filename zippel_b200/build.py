@@ -94,7 +94,7 @@ def build_rowwise(force: bool = False) -> pathlib.Path:
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[a for i in includes for a in ("-isystem", i)], str(src), "-o", str(ROWWISE),
-           "-L", str(libs), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
+           "-L", str(libs), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
            "-L", str(PKG), "-lzippel_b200", "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode:
