@@ -45,12 +45,15 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     if (kJoin) ss.row += ss.step;
     zp_copy_commit();
   };
-  for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
-
-  const bool wide = c.param_dtype == ZP_F32;
   auto column = [&](int i) { return t.piece(i) * V - own.before; };
   // whether the row has any of a thread's piece, and whether there may be a piece that it does not fill
   auto has = [&](int i) { return kFull || (column(i) < width && (kLying != kZpCycled || column(i) + V > 0)); };
+  // whether a thread reads its piece i: but for shifted rows it has zeroes in place of what a row does not have
+  auto reads = [&](int i) { return kLying != kZpShifted || has(i); };
+  if (kLying != kZpShifted && !kFull) zp_clear_pieces<M>(t, ring, ring_bytes / p.slot, p.slot, has);
+  for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
+
+  const bool wide = c.param_dtype == ZP_F32;
   bool edge = false;
 #pragma unroll
   for (int i = 0; i < M && kLying != kZpAligned; ++i) edge = edge || (has(i) && (column(i) < 0 || column(i) + V > width));
@@ -100,7 +103,7 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       float2 s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (turn >= own.n[j] || !has(i)) continue;
+        if (turn >= own.n[j] || !reads(i)) continue;
         zp_read<T, kLying>(t, slot, sx.place_of(j), i, z[j][i]);
         zp_read<T, kLying>(t, slot + p.slot, sy.place_of(j), i, g[j][i]);
         if (kLying != kZpAligned && edge) {    // (a neighbour's elements, or nothing's)
@@ -133,13 +136,13 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       const int64_t at = out + j * next;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (turn >= own.n[j] || !has(i)) continue;
+        if (turn >= own.n[j] || !reads(i)) continue;
         float2 o[H], q[H];
 #pragma unroll
         for (int k = 0; k < H; ++k)
           o[k] = __fmul2_rn(__ffma2_rn(z[j][i][k], minus2, __fadd2_rn(g[j][i][k], minus1)), by);
         if constexpr (!kJoin) {
-          if (c.dx) zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, slot, i, column(i), width, edge, o);
+          if (c.dx && has(i)) zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, slot, i, column(i), width, edge, o);
           continue;
         }
         if (third) {
@@ -147,11 +150,11 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
 #pragma unroll
           for (int k = 0; k < H; ++k) o[k] = __fadd2_rn(o[k], q[k]);
         }
-        if (c.dres) zp_write<T, kLying>(t, static_cast<char *>(c.dres) + at, slot, i, column(i), width, edge, o);
+        if (c.dres && has(i)) zp_write<T, kLying>(t, static_cast<char *>(c.dres) + at, slot, i, column(i), width, edge, o);
         if (!c.dx) continue;
 #pragma unroll
         for (int k = 0; k < H && drops; ++k) o[k] = kept.drop(o[k], i, k, limit, c.drop.scale);
-        zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, slot + p.slot, i, column(i), width, edge, o);
+        if (has(i)) zp_write<T, kLying>(t, static_cast<char *>(c.dx) + at, slot + p.slot, i, column(i), width, edge, o);
       }
     }
     if constexpr (kLying == kZpShifted) {

@@ -40,12 +40,15 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     if (kJoin) sr.row += sr.step;
     zp_copy_commit();
   };
-  for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
-
-  const bool wide = c.param_dtype == ZP_F32;
   auto column = [&](int i) { return t.piece(i) * V - own.before; };
   // whether the row has any of a thread's piece, and whether there may be a piece that it does not fill
   auto has = [&](int i) { return kFull || (column(i) < width && (kLying != kZpCycled || column(i) + V > 0)); };
+  // whether a thread reads its piece i: but for shifted rows it has zeroes in place of what a row does not have
+  auto reads = [&](int i) { return kLying != kZpShifted || has(i); };
+  if (kLying != kZpShifted && !kFull) zp_clear_pieces<M>(t, ring, stages * A * R, p.slot, has);
+  for (int s = 0; s < stages - 1; ++s) fetch(s, ring + s * stage_bytes);
+
+  const bool wide = c.param_dtype == ZP_F32;
   bool edge = false;
 #pragma unroll
   for (int i = 0; i < M && kLying != kZpAligned; ++i) edge = edge || (has(i) && (column(i) < 0 || column(i) + V > width));
@@ -84,7 +87,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (!mine || !has(i)) continue;
+        if (!mine || !reads(i)) continue;
         zp_read<T, kLying>(t, x, sx.place_of(j), i, v[j][i]);
         if constexpr (kJoin) {
           float2 q[H];
@@ -97,14 +100,14 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
           // rounded: what follows works on the sum as it is returned
           const uint4 packed = zp_pack<T>(v[j][i]);
           zp_unpack<T>(packed, v[j][i]);
-          if (kLying != kZpShifted)
+          if (kLying != kZpShifted && has(i))
             zp_write<T, kLying>(t, static_cast<char *>(c.sum) + out + j * next, 0, i, column(i), width, edge, v[j][i]);
         }
       }
       cut(v[j]);
 #pragma unroll
       for (int i = 0; i < M; ++i)
-        if (mine && has(i)) {
+        if (mine && reads(i)) {
 #pragma unroll
           for (int k = 0; k < H; ++k) sum = __fadd2_rn(sum, v[j][i][k]);
         }
@@ -116,10 +119,11 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     for (int j = 0; j < R; ++j) {
       s[j] *= inv_w;
       float2 sq = make_float2(0.f, 0.f);
-      const float2 minus = make_float2(-s[j], -s[j]);
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (turn >= own.n[j] || !has(i)) continue;
+        if (turn >= own.n[j] || !reads(i)) continue;
+        const float less = has(i) ? -s[j] : 0.f;
+        const float2 minus = make_float2(less, less);
         if constexpr (kJoin && kLying == kZpShifted)      // (the team has read all of this slot)
           zp_write<T, kLying>(t, nullptr, slots + j * A * p.slot, i, 0, 0, false, v[j][i]);
 #pragma unroll
@@ -128,7 +132,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       cut(v[j]);
 #pragma unroll
       for (int i = 0; i < M; ++i)
-        if (turn < own.n[j] && has(i)) {
+        if (turn < own.n[j] && reads(i)) {
 #pragma unroll
           for (int k = 0; k < H; ++k) sq = __ffma2_rn(v[j][i][k], v[j][i][k], sq);
         }
@@ -142,7 +146,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
       char *const y = static_cast<char *>(c.y) + out + j * next;
 #pragma unroll
       for (int i = 0; i < M; ++i) {
-        if (turn >= own.n[j] || !has(i)) continue;
+        if (turn >= own.n[j] || !reads(i)) continue;
         float2 (&ww)[H] = w[kHeld ? i : 0], (&bb)[H] = b[kHeld ? i : 0];
         if constexpr (!kHeld) {
           zp_params<T>(c.w, wide, p.vectors, column(i), width, 1.f, ww);
@@ -150,7 +154,8 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
         }
 #pragma unroll
         for (int k = 0; k < H; ++k) v[j][i][k] = __ffma2_rn(__fmul2_rn(v[j][i][k], both), ww[k], bb[k]);
-        zp_write<T, kLying>(t, y, slots + (j * A + A - 1) * p.slot, i, column(i), width, edge, v[j][i]);
+        if (has(i))
+          zp_write<T, kLying>(t, y, slots + (j * A + A - 1) * p.slot, i, column(i), width, edge, v[j][i]);
       }
       if (t.piece(0) == 0 && c.mean && turn < own.n[j]) {
         const int64_t r = own.first + turn * own.step + j * own.next;
