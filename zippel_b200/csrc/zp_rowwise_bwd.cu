@@ -8,7 +8,7 @@
 //
 // B200, both kernels (share of 6 450 GB/s): 8192 x 4096 fp32 66 us (0.94), 16384 x 4096 bf16 74 (0.85; 20 instructions
 // an element, 55 % of the issue slots at sixteen warps: their registers hold the rows, the sums and the weight), joined
-// with dropout 132 (0.79; 41 instructions), 60000 x 128 fp32 19.7 (0.72), 30011 x 1001 fp16 53 (0.53).
+// with dropout 132 (0.79; 41 instructions), 60000 x 128 fp32 19.7 (0.72), 30011 x 1001 fp16 52 (0.54).
 #include "zp_rowwise.cuh"
 
 namespace {

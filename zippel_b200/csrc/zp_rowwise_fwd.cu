@@ -7,7 +7,7 @@
 // B200, one kernel (share of 6 450 GB/s): 8192 x 4096 fp32 43 us (0.97), 16384 x 4096 bf16 48 (0.87; 11.3
 // instructions an element, 46 % of the issue slots: the waits of sixteen warps for each other's sums are what is
 // left), joined with dropout 96 (0.86; 28 instructions, half of them the generator), 60000 x 128 fp32 11.9 (0.80, of it two
-// for the launch and a turn that not every warp has), 30011 x 1001 fp16 40 (0.46: the ends of the rows are the
+// for the launch and a turn that not every warp has), 30011 x 1001 fp16 39 (0.48: the ends of the rows are the
 // work of two lanes while the others wait).
 #include "zp_rowwise.cuh"
 
