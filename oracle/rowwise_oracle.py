@@ -1,4 +1,4 @@
-"""Layer norm, dropout and their residual join in FP64 on the CPU, from their definitions (a checker
+"""Layer norm, dropout and their residual join in FP64 on the CPU, from their definitions (a reference
 for the kernels, never shipped code).  The generator is Philox-4x32-10 (Salmon, Moraes, Dror, Shaw,
 "Parallel random numbers: as easy as 1, 2, 3", SC 2011) in Python's integers."""
 

@@ -3,9 +3,9 @@
     python -m zippel_b200.build [--force] [--verbose]
 
 Each ``csrc/*.cu`` is compiled to an object under ``csrc/_obj`` (skipped when newer than its
-sources) and the objects are linked into ``zippel_b200/libzippel_b200.so``.  ``csrc/*_torch.cpp``, functions
-on torch tensors over that library, become extension modules beside it (``_rowwise``), for the torch and
-Python that build them.
+sources) and the objects are linked into ``zippel_b200/libzippel_b200.so``.  ``csrc/zp_rowwise_torch.cpp``,
+functions on torch tensors over that library, becomes the extension module ``_rowwise`` beside it, for the
+torch and Python that build it.
 """
 
 from __future__ import annotations
@@ -22,6 +22,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = CSRC / "_obj"
 LIB = PKG / "libzippel_b200.so"
+TORCH_SOURCE = CSRC / "zp_rowwise_torch.cpp"      # the operators over rows, on torch tensors
 ROWWISE = PKG / "_rowwise.so"
 
 NVCC_FLAGS = [
@@ -49,6 +50,9 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
     headers = sorted(CSRC.glob("*.cuh")) + sorted((ROOT / "include").glob("*.h"))
     sources = sorted(CSRC.glob("*.cu"))
     jobs = []
+    torch_obj = OBJ / (TORCH_SOURCE.stem + ".o")
+    if force or _stale(torch_obj, [TORCH_SOURCE, ROOT / "include" / "zippel_b200.h"]):
+        jobs.append((TORCH_SOURCE, _torch_compile(torch_obj)))
     for src in sources:
         obj = OBJ / (src.stem + ".o")
         if force or _stale(obj, [src, *headers]):
@@ -68,38 +72,38 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
             if verbose or res.returncode:
                 sys.stderr.write(f"--- {src.name}\n{res.stdout}{res.stderr}\n")
             if res.returncode:
-                raise RuntimeError(f"nvcc failed on {src.name}")
+                raise RuntimeError(f"{'nvcc' if src.suffix == '.cu' else 'g++'} failed on {src.name}")
     objs = [OBJ / (s.stem + ".o") for s in sources]
     if force or jobs or _stale(LIB, objs):
-        cmd = [nvcc(), "-shared", "-o", str(LIB), *map(str, objs), "-lcudart"]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode:
-            raise RuntimeError("link failed:\n" + res.stdout + res.stderr)
-    build_rowwise(force)
+        _link([nvcc(), "-shared", "-o", str(LIB), *map(str, objs), "-lcudart"])
+    if force or _stale(ROWWISE, [torch_obj]):
+        import torch
+        libs = pathlib.Path(torch.__file__).parent / "lib"
+        _link([_gxx(), "-shared", "-o", str(ROWWISE), str(torch_obj), "-L", str(libs), "-ltorch_python", "-ltorch_cuda",
+               "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-L", str(PKG), "-lzippel_b200", "-Wl,-rpath,$ORIGIN"])
     return LIB
 
 
-def build_rowwise(force: bool = False) -> pathlib.Path:
-    """The extension module of the operators over rows (``csrc/zp_rowwise_torch.cpp``)."""
-    src = CSRC / "zp_rowwise_torch.cpp"
-    if not force and not _stale(ROWWISE, [src, ROOT / "include" / "zippel_b200.h"]):
-        return ROWWISE
+def _gxx() -> str:
+    return shutil.which("g++") or "g++"
+
+
+def _torch_compile(obj: pathlib.Path) -> list[str]:
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
     includes = [*cpp_extension.include_paths(), str(pathlib.Path(nvcc()).resolve().parent.parent / "include"),
                 sysconfig.get_paths()["include"], str(ROOT / "include")]
-    libs = pathlib.Path(torch.__file__).parent / "lib"
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[a for i in includes for a in ("-isystem", i)], str(src), "-o", str(ROWWISE),
-           "-L", str(libs), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
-           "-L", str(PKG), "-lzippel_b200", "-Wl,-rpath,$ORIGIN"]
+    return [_gxx(), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[a for i in includes for a in ("-isystem", i)], "-c", str(TORCH_SOURCE), "-o", str(obj)]
+
+
+def _link(cmd: list[str]) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode:
-        raise RuntimeError("g++ failed on " + src.name + ":\n" + res.stdout + res.stderr)
-    return ROWWISE
+        raise RuntimeError("link failed:\n" + res.stdout + res.stderr)
 
 
 if __name__ == "__main__":
