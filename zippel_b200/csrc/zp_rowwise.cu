@@ -89,17 +89,23 @@ dropout_pieces_kernel(int64_t pieces, int rest, int64_t per_row, int64_t rows, i
       for (int i = 0; i < kAhead; ++i)
         if (32 * i < left) in[i] = __ldcs(from + 32 * i);
     } else if constexpr (kHow == kRows) {
-      int64_t q = p0 + lane, r = small ? (uint32_t)q / (uint32_t)per_row : q / per_row;        // row, piece of it
+      int64_t q = p0 + lane;                   // piece of its row
+      const int64_t r = small ? (uint32_t)q / (uint32_t)per_row : q / per_row;
       q -= r * per_row;
+      const T *from = x + r * ldx + q * V;
+      to[0] = y + r * ldy + q * V;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        to[i] = y + r * ldy + q * V;
-        if (32 * i < left) in[i] = __ldcs(reinterpret_cast<const uint4 *>(x + r * ldx + q * V));
+        if (32 * i < left) in[i] = __ldcs(reinterpret_cast<const uint4 *>(from));
+        if (i + 1 == kAhead) break;
         q += 32;
-        if (q >= per_row) {
+        from += 32 * V;
+        to[i + 1] = to[i] + 32 * V;
+        if (q >= per_row) {                    // rows further on
           const int64_t more = per_row >= 32 ? 1 : q / per_row;
-          r += more;
           q -= more * per_row;
+          from += more * (ldx - width);
+          to[i + 1] += more * (ldy - width);
         }
       }
     } else {
