@@ -285,6 +285,31 @@ def test_values_far_from_zero_equal_or_not_finite(dtype):
         assert bool(y[6:].isnan().all())
 
 
+@pytest.mark.parametrize("width", [5, 33, 65, 100, 104, 120, 129, 200])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("extra", [0, 1])
+def test_gradients_of_equal_rows_of_large_values(dtype, width, extra):
+    """Rows of 2^120: their sums are exact, width times fp32(1 / width) is 1 for these widths, so that z is 0 and
+    gx = rstd (gz - mean gz), gw = 0, though mean times rstd is past fp32."""
+    g = torch.Generator().manual_seed(3)
+    gy = torch.randn(20, width, generator=g, dtype=torch.float64).to(dtype)
+    w = (1 + 0.3 * torch.randn(width, generator=g, dtype=torch.float64)).to(dtype)
+    gz = gy.double() * w.double()
+    m = gz.abs().mean(-1, keepdim=True)
+    want = (gz - gz.mean(-1, keepdim=True)) * EPS ** -0.5
+    tol = EPS ** -0.5 * ((width / 32 + 32) * u * m + 6 * u * (gz.abs() + m)) + rounding(dtype, want)
+    base = torch.full((20, width + extra), 2.0 ** 120, dtype=dtype, device="cuda")
+    wc, gc = up(w, gy)
+    x, wc = base[:, :width].detach().requires_grad_(), wc.requires_grad_()
+    rw = rowwise()
+    grads = torch.autograd.grad(rw.layer_norm(x, wc, torch.zeros_like(wc), EPS), (x, wc), gc)
+    near(grads[0], want, tol, "norm")
+    assert not bool(grads[1].any())
+    zero = torch.zeros_like(x)
+    y, _ = rw.dropout_add_layer_norm(zero, x, wc, torch.zeros_like(wc), 0.0, None, EPS)
+    near(torch.autograd.grad(y, x, gc)[0], want, tol, "join")
+
+
 def test_no_rows_and_refusals():
     rw = rowwise()
     x = torch.zeros(0, 16, device="cuda", requires_grad=True)

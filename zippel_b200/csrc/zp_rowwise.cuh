@@ -424,12 +424,12 @@ __device__ __forceinline__ void zp_read(const ZpTeam<kWide> &t, uint32_t slot, i
   const uint32_t at = slot + 16 * (t.lane + i * t.size);
   zp_unpack<T>(kLying == kZpShifted ? zp_read_between<sizeof(T)>(at, place) : zp_lds16(at), v);
 }
-// zeroes in place of what of a piece from column c on lies outside the row
-template <typename T> __device__ __forceinline__ void zp_cut(int c, int width, float2 (&v)[kZpVec<T> / 2]) {
+// `otherwise` in place of what of a piece from column c on lies outside the row
+template <typename T> __device__ __forceinline__ void zp_cut(int c, int width, float2 (&v)[kZpVec<T> / 2], float otherwise) {
 #pragma unroll
   for (int k = 0; k < kZpVec<T> / 2; ++k) {
-    if ((unsigned)(c + 2 * k) >= (unsigned)width) v[k].x = 0.f;
-    if ((unsigned)(c + 2 * k + 1) >= (unsigned)width) v[k].y = 0.f;
+    if ((unsigned)(c + 2 * k) >= (unsigned)width) v[k].x = otherwise;
+    if ((unsigned)(c + 2 * k + 1) >= (unsigned)width) v[k].y = otherwise;
   }
 }
 // Results, piece i from column c on.  `row`: where the team's first piece of the row goes; of a piece that the

@@ -98,7 +98,7 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     float2 z[R][M][H], g[R][M][H];             // normalised rows, and gy w
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const float2 minus = make_float2(-mean[j], -mean[j]), by = make_float2(rstd[j], rstd[j]);
+      const float2 minus = make_float2(-mean[j], -mean[j]);
       const uint32_t slot = slots + j * row_slots;
       float2 s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
@@ -107,9 +107,12 @@ norm_bwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
         zp_read<T, kLying>(t, slot, sx.place_of(j), i, z[j][i]);
         zp_read<T, kLying>(t, slot + p.slot, sy.place_of(j), i, g[j][i]);
         if (kLying != kZpAligned && edge) {    // (a neighbour's elements, or nothing's)
-          zp_cut<T>(column(i), width, z[j][i]);
-          zp_cut<T>(column(i), width, g[j][i]);
+          zp_cut<T>(column(i), width, z[j][i], mean[j]);
+          zp_cut<T>(column(i), width, g[j][i], 0.f);
         }
+        // (z is 0 where the row has nothing: mean times rstd of large and equal values may be infinite)
+        const float scale = has(i) ? rstd[j] : 0.f;
+        const float2 by = make_float2(scale, scale);
 #pragma unroll
         for (int k = 0; k < H; ++k) {
           const float2 zz = __fmul2_rn(__fadd2_rn(z[j][i][k], minus), by), gy = g[j][i][k], gz = __fmul2_rn(gy, w[i][k]);

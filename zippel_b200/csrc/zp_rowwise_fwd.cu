@@ -62,7 +62,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   auto cut = [&](float2 (&v)[M][H]) {
     if (kLying == kZpAligned || !edge) return;
 #pragma unroll
-    for (int i = 0; i < M; ++i) zp_cut<T>(column(i), width, v[i]);
+    for (int i = 0; i < M; ++i) zp_cut<T>(column(i), width, v[i], 0.f);
   };
   const bool drops = kJoin && c.drop.state;
   const ZpPhiloxKey<false> key = drops ? zp_philox_key<false>(c.drop.state) : ZpPhiloxKey<false>{};
