@@ -332,7 +332,7 @@ int zp_layernorm_silu_backward(int64_t rows, int width, const float *x, const fl
  * `state` (device, two int64: seed and offset) and the element's number r * width + c decide: with
  * i = r * width + c, the (i % 8)-th 16-bit half, low half first, of the four words that Philox-4x32-10
  * gives for counter (i / 8, offset) under key `seed` has to be at least t = floor(65536 p + 1/2);
- * keep = 1 - t / 65536.  Nothing is stored: the VJP is the same call on the gradient.  The state is
+ * keep = 1 - t / 65536; t = 0 copies.  Nothing is stored: the VJP is the same call on the gradient.  The state is
  * read when the kernel runs, so a recorded graph follows what is written there between replays.   */
 typedef enum zp_dtype { ZP_F32 = 0, ZP_F16 = 1, ZP_BF16 = 2 } zp_dtype;
 int zp_dropout(int64_t rows, int64_t width, int dtype, const void *x, int64_t ldx, double p,
