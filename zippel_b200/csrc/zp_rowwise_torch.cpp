@@ -111,21 +111,26 @@ struct Rows {                       // `t`: the tensor or a copy that the kernel
   const void *data() const { return t.const_data_ptr(); }
 };
 
+// Rows that lie ld >= width elements apart are read where they are.  All others come from a copy, among them rows that
+// are one row repeated (a stride of 0, as the gradient of a sum over rows has it) and rows that overlap.
 Rows rows_of(const Tensor &x) {
-  const int64_t w = x.dim() ? x.size(-1) : 1;
-  if (x.is_contiguous()) return {x, w ? x.numel() / w : 0, w, w};
-  if (x.numel() && (x.stride(-1) == 1 || w == 1)) {          // leading axes one row behind the other
-    int64_t ld = 0, next = 0;
-    bool fits = true;
-    for (int64_t i = x.dim() - 2; i >= 0 && fits; --i) {
-      if (x.size(i) == 1) continue;
-      if (!ld) ld = x.stride(i);
-      else fits = x.stride(i) == next;
-      next = x.stride(i) * x.size(i);
+  const int64_t w = x.dim() ? x.size(-1) : 1, rows = w ? x.numel() / w : 0;
+  if (x.is_contiguous()) return {x, rows, w, w};
+  bool fits = x.numel() && (x.stride(-1) == 1 || w == 1), found = false;
+  int64_t ld = w, next = 0;
+  for (int64_t i = x.dim() - 2; i >= 0 && fits; --i) {       // leading axes one row behind the other
+    if (x.size(i) == 1) continue;
+    if (!found) {
+      found = true;
+      ld = x.stride(i);
+      fits = ld >= w;
+    } else {
+      fits = x.stride(i) == next;
     }
-    if (fits && (ld >= w || !ld)) return {x, x.numel() / w, w, ld ? ld : w};
+    next = x.stride(i) * x.size(i);
   }
-  return {x.contiguous(), w ? x.numel() / w : 0, w, w};
+  if (fits) return {x, rows, w, ld};
+  return {x.contiguous(), rows, w, w};
 }
 
 // new arrays, without the dispatcher's detour (0.5 us each)
@@ -394,12 +399,22 @@ ENTRY(dropout_add_layer_norm, 7,
       const double eps = number_arg(a[6]),
       dropout_add_layer_norm(x, residual, w, b, p, state, eps), pair)
 
+// (rows, width, ld, whether they are a copy's) of a tensor as the functions above read it, on whatever device
+PyObject *py_row_layout(PyObject *, PyObject *a) {
+  HANDLE_TH_ERRORS
+  const Tensor x = tensor_arg(a, "x");
+  const Rows r = rows_of(x);
+  return Py_BuildValue("LLLN", (long long)r.rows, (long long)r.width, (long long)r.ld, PyBool_FromLong(!r.t.is_same(x)));
+  END_HANDLE_TH_ERRORS
+}
+
 template <typename F> PyCFunction fast(F *f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(f)); }
 PyMethodDef methods[] = {
     {"layer_norm", fast(py_layer_norm), METH_FASTCALL, "layer_norm(x, weight, bias, eps)"},
     {"dropout", fast(py_dropout), METH_FASTCALL, "dropout(x, p, state)"},
     {"dropout_add_layer_norm", fast(py_dropout_add_layer_norm), METH_FASTCALL,
      "dropout_add_layer_norm(x, residual, weight, bias, p, state, eps)"},
+    {"row_layout", py_row_layout, METH_O, "row_layout(x): (rows, width, ld, copied)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_rowwise", nullptr, -1, methods};
 
