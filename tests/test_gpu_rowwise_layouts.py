@@ -115,3 +115,26 @@ def test_gradients_of_sums_over_rows(over, width, dtype):
     near(got[0].view(rows, width), want.gx * f, (want.line + 3 * u * want.gx.abs()) * f + rounding(dtype, want.gx * f), "x")
     near(got[2], want.gw, want.tgw, "weight")
     near(got[3], want.gb, want.tgb, "bias")
+
+
+@pytest.mark.parametrize("width", [1, 24])
+def test_lazy_negations_and_zeroes(width):
+    """Rows, parameters and gradients whose values are not what lies in memory."""
+    g = torch.Generator("cuda").manual_seed(1)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda")                    # noqa: E731
+    if width == 1:
+        lazy = [torch.complex(new(*s), new(*s)).conj().imag for s in [(40, 1)] * 4 + [(1,)] * 2]
+    else:
+        lazy = [torch._neg_view(new(*s)) for s in [(40, width)] * 4 + [(width,)] * 2]
+    assert all(t.is_neg() for t in lazy)
+    order = lambda t: (t[0], t[1], t[4], t[5], t[2], t[3])                          # noqa: E731
+    plain = [t.clone(memory_format=torch.contiguous_format) for t in lazy]
+    assert not any(t.is_neg() for t in plain)
+    same(calls(*order(lazy)), calls(*order(plain)), plain[2])
+
+    leaves = [t.clone().requires_grad_() for t in (plain[0], plain[1])]
+    ys = rowwise().dropout_add_layer_norm(*leaves, None, None, 0.3, torch.tensor([5, 6], device="cuda"))
+    zero = torch._efficientzerotensor((40, width), device="cuda")
+    got = torch.autograd.grad(ys, leaves, [zero, plain[3]], retain_graph=True)
+    want = torch.autograd.grad(ys, leaves, [torch.zeros(40, width, device="cuda"), plain[3]])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

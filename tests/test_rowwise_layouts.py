@@ -107,3 +107,19 @@ def test_random_strides(row_layout):
         if 7 + sum((n - 1) * s for n, s in zip(shape, strides)) >= base.numel():
             continue
         check(row_layout, base.as_strided(shape, strides, 7), None)
+
+
+def lazy_tensors():
+    z = torch.complex(new(A, W), -new(A, W)).conj()
+    return {"negated": torch._neg_view(new(A, W)), "negated, one axis": torch._neg_view(new(W)),
+            "a column of imaginary parts": z[:, :1].imag, "an imaginary part": z[:1, :1].imag,
+            "imaginary parts": z.imag, "negated rows of a wider array": torch._neg_view(new(A, W + 5)[:, :W]),
+            "zeroes that are not stored": torch._efficientzerotensor((A, W))}
+
+
+@pytest.mark.parametrize("name", lazy_tensors())
+def test_values_that_are_not_in_memory_come_from_a_copy(row_layout, name):
+    """Lazy negations and zeroes without storage: what lies at the tensor's address is not its values."""
+    x = lazy_tensors()[name]
+    rows, width, ld, copied = row_layout(x)
+    assert copied and (rows, width) == (x.numel() // x.shape[-1], x.shape[-1]) and ld >= width

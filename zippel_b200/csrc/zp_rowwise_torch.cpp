@@ -89,7 +89,8 @@ bool need_drop(const Tensor &x, double p, const Tensor &state) {
   TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "a probability is between 0 and 1: ", p);
   if (std::floor(65536.0 * p + 0.5) == 0.0) return false;
   TORCH_CHECK_VALUE(state.defined(), "dropout with p > 0 needs a state: dropout_state(device) draws one");
-  TORCH_CHECK_VALUE(state.scalar_type() == at::kLong && state.dim() == 1 && state.size(0) == 2 && state.is_contiguous(),
+  TORCH_CHECK_VALUE(state.scalar_type() == at::kLong && state.dim() == 1 && state.size(0) == 2 && state.is_contiguous() &&
+                        !state.is_neg(),
                     "a dropout state is two int64 one behind the other (seed, offset)");
   TORCH_CHECK(state.device() == x.device(), "the dropout state is on ", state.device(), ", x on ", x.device());
   return true;
@@ -111,10 +112,15 @@ struct Rows {                       // `t`: the tensor or a copy that the kernel
   const void *data() const { return t.const_data_ptr(); }
 };
 
+// Whether what lies in memory is not the tensor's values: they are negated (imaginary parts of a conjugate), or zeroes
+// that are not stored.  A clone has them in memory.
+bool lazy(const Tensor &x) { return x.is_neg() || x._is_zerotensor(); }
+
 // Rows that lie ld >= width elements apart are read where they are.  All others come from a copy, among them rows that
 // are one row repeated (a stride of 0, as the gradient of a sum over rows has it) and rows that overlap.
 Rows rows_of(const Tensor &x) {
   const int64_t w = x.dim() ? x.size(-1) : 1, rows = w ? x.numel() / w : 0;
+  if (lazy(x)) return rows_of(x.clone());
   if (x.is_contiguous()) return {x, rows, w, w};
   bool fits = x.numel() && (x.stride(-1) == 1 || w == 1), found = false;
   int64_t ld = w, next = 0;
@@ -138,7 +144,9 @@ Tensor array(at::IntArrayRef sizes, at::ScalarType type, const Tensor &beside) {
   return at::detail::empty_cuda(sizes, type, beside.device(), std::nullopt);
 }
 Tensor like(const Tensor &x) { return array(x.sizes(), x.scalar_type(), x); }    // row behind row
-Tensor lined_up(const Tensor &t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
+Tensor lined_up(const Tensor &t) {
+  return t.defined() && (!t.is_contiguous() || lazy(t)) ? t.clone(at::MemoryFormat::Contiguous) : t;
+}
 const void *address(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void *room(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 const int64_t *state_of(const Tensor &t) { return static_cast<const int64_t *>(address(t)); }
