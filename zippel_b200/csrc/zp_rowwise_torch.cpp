@@ -8,7 +8,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -54,7 +56,16 @@ int type_number(at::ScalarType t) {
   return t == at::kFloat ? ZP_F32 : t == at::kHalf ? ZP_F16 : t == at::kBFloat16 ? ZP_BF16 : -1;
 }
 
+// A tracer records what goes through torch's dispatcher, which these calls do not: their results would be constants of
+// the trace.
+void need_no_trace(const char *what) {
+  TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled() &&
+                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+              what, " leaves nothing in a trace: torch.jit.trace and make_fx cannot record it");
+}
+
 int need_rows(const Tensor &x, const char *what) {
+  need_no_trace(what);
   TORCH_CHECK(x.is_cuda(), what, " needs CUDA tensors: there is no CPU path");
   const int type = type_number(x.scalar_type());
   TORCH_CHECK_TYPE(type >= 0, what, " takes float32, float16 and bfloat16, not ", x.scalar_type());
