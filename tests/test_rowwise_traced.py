@@ -1,4 +1,5 @@
-"""Calls of the operators over rows under torch's tracers, which would keep their result as a constant: refused."""
+"""Calls of the operators over rows under torch's tracers, which would keep their result as a constant, and of tensors that
+torch wraps without giving them memory: refused."""
 
 from __future__ import annotations
 
@@ -55,3 +56,20 @@ def test_a_trace_elsewhere_refuses_nothing(name):
 
     make_fx(traced)(x)
     assert torch.equal(got[0], want)
+
+
+@pytest.mark.gpu
+def test_tensors_without_memory_are_refused():
+    """A wrapped weight is not a missing one, nor a wrapped residual or state."""
+    from zippel_b200.blocks import rowwise as rw
+    x, w = torch.randn(4, 8, device="cuda"), torch.full((8,), 3.0, device="cuda")
+    state, wrapped = torch.tensor([1, 2], device="cuda"), torch.func.functionalize
+    for call in (lambda: wrapped(lambda v: rw.layer_norm(x, v))(w), lambda: wrapped(lambda v: rw.layer_norm(x, None, v))(w),
+                 lambda: wrapped(lambda v: rw.layer_norm(v, w))(x), lambda: wrapped(lambda v: rw.dropout(v, 0.5, state))(x),
+                 lambda: wrapped(lambda v: rw.dropout(x, 0.5, v))(state),
+                 lambda: wrapped(lambda v: rw.dropout_add_layer_norm(x, v, w, w))(x),
+                 lambda: wrapped(lambda v: rw.dropout_add_layer_norm(v, x, w, w)[0])(x),
+                 lambda: wrapped(lambda v: rw.dropout_add_layer_norm(x, x, v, w)[0])(w),
+                 lambda: wrapped(lambda v: rw.dropout_add_layer_norm(x, x, w, w, 0.5, v)[0])(state)):
+        with pytest.raises(RuntimeError, match="no memory of its own"):
+            call()

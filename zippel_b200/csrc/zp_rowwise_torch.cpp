@@ -117,10 +117,19 @@ bool recorded(std::initializer_list<const Tensor *> tensors) {
 
 // ---- layout ---------------------------------------------------------------------------------------
 
+// What the kernels read.  A wrapped tensor without memory (a functionalized one has a null address) is not one that
+// is missing.
+const void *address(const Tensor &t) {
+  if (!t.defined() || !t.numel()) return nullptr;
+  const void *p = t.const_data_ptr();
+  TORCH_CHECK(p, "a tensor of shape ", t.sizes(), " has no memory of its own: it is wrapped, or zeroes that are not stored");
+  return p;
+}
+
 struct Rows {                       // `t`: the tensor or a copy that the kernels can read
   Tensor t;
   int64_t rows, width, ld;
-  const void *data() const { return t.const_data_ptr(); }
+  const void *data() const { return address(t); }
 };
 
 // Whether what lies in memory is not the tensor's values: they are negated (imaginary parts of a conjugate), or zeroes
@@ -158,7 +167,6 @@ Tensor like(const Tensor &x) { return array(x.sizes(), x.scalar_type(), x); }   
 Tensor lined_up(const Tensor &t) {
   return t.defined() && (!t.is_contiguous() || lazy(t)) ? t.clone(at::MemoryFormat::Contiguous) : t;
 }
-const void *address(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void *room(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 const int64_t *state_of(const Tensor &t) { return static_cast<const int64_t *>(address(t)); }
 
