@@ -570,7 +570,7 @@ struct ZpTeamPlan {
   bool full, vectors;
   int slot, bytes, stages;                     // bytes of a slot, of the counters' bits of a team
   size_t smem;
-  unsigned blocks;
+  unsigned blocks;                             // 0 once a device has been found to run none of the plan's clusters
 };
 // The largest number of teams up to `most` of which every class of the cycle has as many
 inline int64_t zp_whole_cycles(const ZpTeamPlan &p, int64_t most) {
@@ -617,11 +617,13 @@ inline bool zp_team_plan(const ZpNormCall &c, int lying, int arrays, size_t last
   p.blocks = (unsigned)(own * p.ranks);
   return true;
 }
-// Clusters of `kernel` that run at the same time, looked up once per device and size
+// Clusters of `kernel` that run at the same time, looked up once per device and size (0: none, asked for anew)
 struct ZpClusters {
   std::mutex lock;
   int most[64][4] = {};
 };
+// The plan's blocks as far as the device runs their clusters at the same time.  None: not even one of every class of
+// the cycle.
 template <typename Kernel> int zp_fit_clusters(Kernel kernel, ZpTeamPlan &p, ZpClusters &state) {
   int dev = 0, log = p.ranks == 2 ? 1 : p.ranks == 4 ? 2 : 3;
   ZP_CUDA(cudaGetDevice(&dev));
@@ -636,18 +638,19 @@ template <typename Kernel> int zp_fit_clusters(Kernel kernel, ZpTeamPlan &p, ZpC
     cfg.gridDim = dim3(148 / p.ranks * p.ranks); cfg.blockDim = dim3(kZpTeamThreads); cfg.dynamicSmemBytes = 227 * 1024;
     cfg.attrs = attr; cfg.numAttrs = 1;
     ZP_CUDA(cudaOccupancyMaxActiveClusters(&most, kernel, &cfg));
-    if (most < 8) return ZP_ERR_UNSUPPORTED;
   }
   if ((int64_t)p.blocks > (int64_t)most * p.ranks) p.blocks = (unsigned)(zp_whole_cycles(p, most) * p.ranks);
   return ZP_OK;
 }
-// One kernel of teams; kWide: teams are clusters
+// One kernel of teams; kWide: teams are clusters.  A plan that is left without blocks is not launched.
 template <bool kWide, typename Kernel>
 int zp_launch_teams(Kernel kernel, const char *name, const ZpNormCall &c, ZpTeamPlan &p, ZpSmemOptIn &opt_in,
                     ZpClusters &clusters, cudaStream_t st) {
   if (int rc = zp_ensure_smem(kernel, kWide ? 227 * 1024 : p.smem, opt_in)) return rc;
-  if constexpr (kWide)
+  if constexpr (kWide) {
     if (int rc = zp_fit_clusters(kernel, p, clusters)) return rc;
+    if (p.blocks == 0) return ZP_OK;
+  }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -289,6 +289,7 @@ int zp_launch_norm_bwd(const ZpNormCall &c, bool &taken, int &parts, cudaStream_
   const int rc = c.dtype == ZP_F32   ? by_kind<float>(c, p, st)
                  : c.dtype == ZP_F16 ? by_kind<__half>(c, p, st)
                                      : by_kind<__nv_bfloat16>(c, p, st);
+  taken = p.blocks > 0;
   parts = (int)p.blocks / p.ranks;
   return rc;
 }

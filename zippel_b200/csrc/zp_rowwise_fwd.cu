@@ -235,7 +235,9 @@ int zp_launch_norm_fwd(const ZpNormCall &c, bool &taken, cudaStream_t st) {
           ((wide || each >= 32 || span > 8 * kZpTeamThreads) && zp_team_plan(c, lying, arrays, 0, 16, 1, p)) ||
           (!wide && zp_team_plan(c, lying, arrays, 0, 8, 1, p) && p.ranks == 1);
   if (!taken) return ZP_OK;
-  if (c.dtype == ZP_F32) return by_kind<float>(c, p, st);
-  if (c.dtype == ZP_F16) return by_kind<__half>(c, p, st);
-  return by_kind<__nv_bfloat16>(c, p, st);
+  const int rc = c.dtype == ZP_F32   ? by_kind<float>(c, p, st)
+                 : c.dtype == ZP_F16 ? by_kind<__half>(c, p, st)
+                                     : by_kind<__nv_bfloat16>(c, p, st);
+  taken = p.blocks > 0;
+  return rc;
 }
