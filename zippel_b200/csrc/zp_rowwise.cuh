@@ -18,6 +18,7 @@
 //                  thread puts its pieces together from two of them, and results go the same way back
 #pragma once
 
+#include <cmath>
 #include <initializer_list>
 #include <utility>
 
@@ -561,6 +562,18 @@ template <typename T, int kLying, bool kWords, int E> struct ZpKept {
 
 // ---- launches ---------------------------------------------------------------------------------------
 
+// One over a width as a float and what that lacks: `one` is off by at most half a step, 1 - one W is a float (fmaf gives
+// it without a rounding), and one + rest is 1/W within 2^-47.  So a sum that is the width times a float gives
+// exactly that float: with `one` alone rows of equal values had z 0.02 in place of 0 (1000 columns, or 41, of 1000.0).
+struct ZpOver {
+  float one, rest;
+  __host__ __device__ __forceinline__ float of(float sum) const { return fmaf(sum, one, sum * rest); }
+};
+inline ZpOver zp_over(int64_t width) {
+  const float one = 1.f / (float)width;
+  return {one, fmaf(-one, (float)width, 1.f) * one};
+}
+
 // How a call's rows are shared out: elements per thread and rows at a time, the team's size, how the rows
 // lie, whether every thread has all its pieces, whether weight and bias lie in aligned ones, and the ring's sizes.
 struct ZpTeamPlan {
@@ -570,6 +583,7 @@ struct ZpTeamPlan {
   bool full, vectors;
   int slot, bytes, stages;                     // bytes of a slot, of the counters' bits of a team
   size_t smem;
+  ZpOver over;                                 // the width
   unsigned blocks;                             // 0 once a device has been found to run none of the plan's clusters
 };
 // The largest number of teams up to `most` of which every class of the cycle has as many
@@ -594,6 +608,7 @@ inline bool zp_team_plan(const ZpNormCall &c, int lying, int arrays, size_t last
   p.cycle = lying != kZpCycled ? 1 : c.width % 2 ? 8 : c.width % 4 ? 4 : 2;
   p.vectors = lying != kZpCycled && c.width % (16 / size) == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0 &&
               reinterpret_cast<uintptr_t>(c.b) % 16 == 0;
+  p.over = zp_over(c.width);
   p.elements = elements;
   p.rows = rows;
   const int64_t need = p.ranks > 1 ? kZpTeamThreads : zp_ceil_div(span, elements);

@@ -67,7 +67,8 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
   const bool drops = kJoin && c.drop.state;
   const ZpPhiloxKey<false> key = drops ? zp_philox_key<false>(c.drop.state) : ZpPhiloxKey<false>{};
   const uint32_t limit = zp_drop_limit(c.drop.threshold);
-  const float inv_w = 1.f / (float)width;
+  // (worked out here: read from the parameters it makes fp32 rows of odd width 3 % slower, 20000 x 1001 32.4 us -> 33.2)
+  const ZpOver over = {1.f / (float)width, p.over.rest};
   const int64_t row_bytes = c.width * (int64_t)sizeof(T), next = own.next * row_bytes;
   int64_t out = own.first * row_bytes - own.before * (int)sizeof(T);        // of the rows that are worked on, in every result
   t.meet();                                    // the team's blocks run
@@ -117,7 +118,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     float q[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      s[j] *= inv_w;
+      s[j] = over.of(s[j]);
       float2 sq = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < M; ++i) {
@@ -141,7 +142,7 @@ norm_fwd_team_kernel(const __grid_constant__ ZpNormCall c, const __grid_constant
     t.sum(q, 1, kLying == kZpShifted);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const float rstd = rsqrtf(q[j] * inv_w + c.eps);
+      const float rstd = rsqrtf(q[j] * over.one + c.eps);
       const float2 both = make_float2(rstd, rstd);
       char *const y = static_cast<char *>(c.y) + out + j * next;
 #pragma unroll
