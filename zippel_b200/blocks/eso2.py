@@ -712,13 +712,16 @@ def radial_mlp(plan: Plan, x_edge: torch.Tensor, layers: list) -> torch.Tensor:
         elif isinstance(m, nn.Linear):
             h = tensor_core_linear(plan, h, m.weight, m.bias) if h.shape[0] else h.new_zeros(0, m.out_features)
             i += 1
-        elif isinstance(m, nn.LayerNorm) and i + 1 < len(layers) and isinstance(layers[i + 1], nn.SiLU):
-            h = LayerNormSiLU.apply(h, m.weight, m.bias, m.eps) if h.shape[0] else h
-            i += 2
         elif isinstance(m, nn.LayerNorm) and len(m.normalized_shape) == 1:
-            params = [None if t is None else t.to(h.dtype) for t in (m.weight, m.bias)]
-            h = rowwise.layer_norm(h, *params, m.eps)
-            i += 1
+            if m.normalized_shape[0] != h.shape[-1]:
+                raise ValueError(f"LayerNorm({m.normalized_shape[0]}) on rows of {h.shape[-1]} channels")
+            if i + 1 < len(layers) and isinstance(layers[i + 1], nn.SiLU):
+                h = LayerNormSiLU.apply(h, m.weight, m.bias, m.eps) if h.shape[0] else h
+                i += 2
+            else:
+                params = [None if t is None else t.to(h.dtype) for t in (m.weight, m.bias)]
+                h = rowwise.layer_norm(h, *params, m.eps)
+                i += 1
         elif isinstance(m, nn.Dropout):
             if m.training and m.p > 0:
                 h = rowwise.dropout(h, m.p, rowwise.dropout_state(h.device))
