@@ -457,9 +457,12 @@ class TensorCoreLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan: Plan, x, weight, bias):
         lib = _lib.load()
+        m, k = x.shape
+        n = weight.shape[0]
+        if weight.shape != (n, k) or bias.shape != (n,):     # (the kernels read as many as these sizes say)
+            raise ValueError(f"a linear layer with a weight {tuple(weight.shape)} and a bias {tuple(bias.shape)} on rows "
+                             f"of {k} channels")
         xf, wf, bf = _f32(x), _f32(weight), _f32(bias)
-        m, k = xf.shape
-        n = wf.shape[0]
         y = torch.empty(m, n, dtype=torch.float32, device=xf.device)
         nbytes = lib.zp_linear_work_bytes(plan.handle, m, k, n)
         if nbytes == 0:
@@ -514,10 +517,13 @@ class LayerNormSiLU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, eps: float):
         lib = _lib.load()
+        rows, width = x.shape
+        if gamma.shape != (width,) or beta.shape != (width,):
+            raise ValueError(f"LayerNormSiLU with parameters {tuple(gamma.shape)} and {tuple(beta.shape)} on rows of "
+                             f"{width} channels")
         if not x.is_cuda:
             raise RuntimeError("LayerNormSiLU needs CUDA tensors: there is no CPU path")
         xf, gf, bf = _f32(x), _f32(gamma), _f32(beta)
-        rows, width = xf.shape
         y = torch.empty_like(xf)
         stats = torch.empty(2, rows, dtype=torch.float32, device=xf.device)
         with torch.cuda.device(xf.device):
@@ -682,6 +688,8 @@ def tensor_core_linear(plan: Plan, x: torch.Tensor, weight: torch.Tensor, bias) 
     """``x @ weight.T + bias`` through ``TensorCoreLinear`` for any sizes: the engine wants inner
     and outer widths in multiples of 8, so odd ones are zero-padded (and the result sliced)."""
     n_out, n_in = weight.shape
+    if x.shape[1] != n_in:
+        raise ValueError(f"a linear layer of {n_in} channels on rows of {x.shape[1]}")
     pad_in, pad_out = (-n_in) % 8, (-n_out) % 8
     if bias is None:
         bias = weight.new_zeros(n_out)
