@@ -45,3 +45,36 @@ def test_a_norm_with_parameters_of_another_width(shape):
     for gamma, beta in ((other, other), (fit, other), (other, fit)):
         with pytest.raises(ValueError, match="32"):
             run([("ln_silu", gamma, beta, 1e-5)])
+
+
+def test_a_norm_without_parameters_in_front_of_a_silu_is_not_refused_for_them():
+    """(The refusal that is left is that there is no CPU path.)"""
+    for norm in (nn.LayerNorm(32, elementwise_affine=False), nn.LayerNorm(32, bias=False)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            run([norm, nn.SiLU()])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["no parameters", "no bias"])
+def test_a_norm_without_parameters_in_front_of_a_silu(kind):
+    """Values and gradients within 1e-5 of the same layers in FP64, the bound that this package's tests hold its fp32
+    path to."""
+    import copy
+
+    from tests.helpers import rel_l2
+    from zippel_b200.blocks.eso2 import Plan, radial_mlp
+    torch.manual_seed(0)
+    norm = nn.LayerNorm(32, elementwise_affine=False) if kind == "no parameters" else nn.LayerNorm(32, bias=False)
+    layers = nn.Sequential(nn.Linear(16, 32), norm, nn.SiLU(), nn.Linear(32, 24)).cuda()
+    if kind == "no bias":
+        nn.init.normal_(norm.weight)
+    x, up = torch.randn(100, 16, device="cuda", requires_grad=True), torch.randn(100, 24, device="cuda")
+    y = radial_mlp(Plan.get(2, 1, 16, 16, x.device), x, list(layers))
+    got = torch.autograd.grad(y, [x, *layers.parameters()], up)
+    ref = copy.deepcopy(layers).cpu().double()
+    x64 = x.detach().cpu().double().requires_grad_()
+    y64 = ref(x64)
+    want = torch.autograd.grad(y64, [x64, *ref.parameters()], up.cpu().double())
+    assert rel_l2(y, y64) < 1e-5
+    for g, r in zip(got, want, strict=True):
+        assert rel_l2(g, r) < 1e-5

@@ -724,7 +724,9 @@ def radial_mlp(plan: Plan, x_edge: torch.Tensor, layers: list) -> torch.Tensor:
             if m.normalized_shape[0] != h.shape[-1]:
                 raise ValueError(f"LayerNorm({m.normalized_shape[0]}) on rows of {h.shape[-1]} channels")
             if i + 1 < len(layers) and isinstance(layers[i + 1], nn.SiLU):
-                h = LayerNormSiLU.apply(h, m.weight, m.bias, m.eps) if h.shape[0] else h
+                gamma = h.new_ones(h.shape[-1]) if m.weight is None else m.weight
+                beta = h.new_zeros(h.shape[-1]) if m.bias is None else m.bias
+                h = LayerNormSiLU.apply(h, gamma, beta, m.eps) if h.shape[0] else h
                 i += 2
             else:
                 params = [None if t is None else t.to(h.dtype) for t in (m.weight, m.bias)]
