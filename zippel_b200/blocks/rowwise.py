@@ -35,7 +35,11 @@ def _native():
     global _module
     if _module is None:
         _lib.load()                            # (says what to do where nothing has been built)
-        from .. import _rowwise as _module
+        try:
+            from .. import _rowwise as _module
+        except ImportError as e:               # built without a torch, or for another one
+            raise RuntimeError("the functions on tensors are missing or for another torch: build them with "
+                               f"`python -m zippel_b200.build` ({e})") from e
     return _module
 
 

@@ -5,12 +5,14 @@
 Each ``csrc/*.cu`` is compiled to an object under ``csrc/_obj`` (skipped when newer than its
 sources) and the objects are linked into ``zippel_b200/libzippel_b200.so``.  ``csrc/zp_rowwise_torch.cpp``,
 functions on torch tensors over that library, becomes the extension module ``_rowwise`` beside it, for the
-torch and Python that build it.
+torch and Python that build it (and anew for others); where there is no torch for CUDA it is left out.
 """
 
 from __future__ import annotations
 
 import concurrent.futures
+import importlib.metadata
+import importlib.util
 import os
 import pathlib
 import shutil
@@ -50,8 +52,12 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
     headers = sorted(CSRC.glob("*.cuh")) + sorted((ROOT / "include").glob("*.h"))
     sources = sorted(CSRC.glob("*.cu"))
     jobs = []
-    torch_obj = OBJ / (TORCH_SOURCE.stem + ".o")
-    if force or _stale(torch_obj, [TORCH_SOURCE, ROOT / "include" / "zippel_b200.h"]):
+    torch_obj, made_for = OBJ / (TORCH_SOURCE.stem + ".o"), _made_for()
+    if made_for is None:
+        print("no torch for CUDA is installed: the functions on tensors (blocks/rowwise.py) are left out", file=sys.stderr)
+    elif (force or _stale(torch_obj, [TORCH_SOURCE, ROOT / "include" / "zippel_b200.h"])
+          or not _stamp().exists() or _stamp().read_text() != made_for):
+        _stamp().unlink(missing_ok=True)
         jobs.append((TORCH_SOURCE, _torch_compile(torch_obj)))
     for src in sources:
         obj = OBJ / (src.stem + ".o")
@@ -74,14 +80,32 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
             if res.returncode:
                 raise RuntimeError(f"{'nvcc' if src.suffix == '.cu' else 'g++'} failed on {src.name}")
     objs = [OBJ / (s.stem + ".o") for s in sources]
-    if force or jobs or _stale(LIB, objs):
+    if force or _stale(LIB, objs):
         _link([nvcc(), "-shared", "-o", str(LIB), *map(str, objs), "-lcudart"])
-    if force or _stale(ROWWISE, [torch_obj]):
+    if made_for is not None and (force or _stale(ROWWISE, [torch_obj]) or not _stamp().exists()):
         import torch
         libs = pathlib.Path(torch.__file__).parent / "lib"
         _link([_gxx(), "-shared", "-o", str(ROWWISE), str(torch_obj), "-L", str(libs), "-ltorch_python", "-ltorch_cuda",
-               "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-L", str(PKG), "-lzippel_b200", "-Wl,-rpath,$ORIGIN"])
+               "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10", "-L", str(LIB.parent), "-lzippel_b200", "-Wl,-rpath,$ORIGIN"])
+        _stamp().write_text(made_for)
     return LIB
+
+
+def _made_for() -> str | None:
+    """The torch and Python that an extension built now fits; None without a torch for CUDA."""
+    torch = importlib.util.find_spec("torch")
+    if torch is None or not (pathlib.Path(torch.origin).parent / "lib" / "libc10_cuda.so").exists():
+        return None
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:          # (one that was not installed as a package)
+        version = torch.origin
+    return f"torch {version}, Python {sys.version}"
+
+
+def _stamp() -> pathlib.Path:
+    """Holds what the extension was last built for."""
+    return OBJ / (TORCH_SOURCE.stem + ".for")
 
 
 def _gxx() -> str:
