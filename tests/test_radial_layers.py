@@ -78,3 +78,28 @@ def test_a_norm_without_parameters_in_front_of_a_silu(kind):
     assert rel_l2(y, y64) < 1e-5
     for g, r in zip(got, want, strict=True):
         assert rel_l2(g, r) < 1e-5
+
+
+STACKS = {"dropout for silu": lambda c, w: [nn.Linear(w, c), nn.LayerNorm(c), nn.Dropout(0.1), nn.Linear(c, c),
+                                             nn.LayerNorm(c), nn.SiLU()],
+          "residual layers": lambda c, w: [nn.Linear(w, c), nn.LayerNorm(c), nn.SiLU(), residual([nn.Linear(c, c)], c),
+                                            nn.LayerNorm(c), nn.SiLU()],
+          "one layer more": lambda c, w: [nn.Linear(w, c), nn.LayerNorm(c), nn.SiLU(), nn.Linear(c, c), nn.LayerNorm(c),
+                                           nn.SiLU(), nn.Linear(c, c), nn.Dropout(0.1)],
+          "another eps": lambda c, w: [nn.Linear(w, c), nn.LayerNorm(c, eps=1e-3), nn.SiLU(), nn.Linear(c, c),
+                                        nn.LayerNorm(c), nn.SiLU()]}
+
+
+@pytest.mark.parametrize("name", STACKS)
+def test_a_program_is_not_bound_to_other_layers(name):
+    """The programs have the reference's radial MLP written out, eps 1e-5 included."""
+    from tests.helpers import random_case
+    from zippel_b200.blocks.eso2 import BlockConfig, ESO2Block, load_jd
+    from zippel_b200.blocks.ir_bind import bind
+    cfg = dict(lmax=2, mmax=1, sphere_channels=8, hidden_channels=8, edge_channels=16, num_distance_basis=8, cutoff=5.0)
+    block, case = ESO2Block(BlockConfig(**cfg)), random_case(cfg, 6, 20, seed=1)
+    bind(block, case, load_jd(2))
+    last = block.rad_func[-1]
+    block.rad_func = nn.Sequential(*STACKS[name](16, block.rad_func[0].in_features), last)
+    with pytest.raises(ValueError, match="radial"):
+        bind(block, case, load_jd(2))

@@ -3,14 +3,15 @@
 Same contract as the reference's ``blocks/ir_bind.py:26-103``: ``bind(block, batch, jd_list, cfg)
 -> (inputs, sizes)`` with every value tensor carrying a leading segment axis (length 1 for shared
 parameters), FP64 on the CPU.  ``block`` may be an ``ESO2Block`` or a reference ``ESO2RefBlock``
-(same parameter names).  ``to_m`` is the rectangular ``[1, Km, K]`` selection.
+(same parameter names), with the radial MLP that it was made with: other layers are refused.
+``to_m`` is the rectangular ``[1, Km, K]`` selection.
 """
 
 from __future__ import annotations
 
 import torch
 
-from .eso2 import BlockConfig, Layout
+from .eso2 import _RADIAL_LAYERS, BlockConfig, Layout
 
 DT = torch.float64
 
@@ -43,7 +44,11 @@ def bind(block, batch, jd_list, cfg: BlockConfig | None = None):
         "gauss_offset": t(block.gauss_offset).unsqueeze(0), "ones_g": one(1, NB), "ones": one(e),
         "unit": one(1, 1), "unit_mat": one(1, 1, 1), "unit_m": one(1, 1), "ones_ec": one(1, EC),
     }
-    rad = block.rad_func
+    rad = list(block.rad_func)
+    if (len(rad) != len(_RADIAL_LAYERS) or not all(map(isinstance, rad, _RADIAL_LAYERS))
+            or rad[1].eps != 1e-5 or rad[4].eps != 1e-5):
+        raise ValueError("the programs have the reference's radial MLP written out (Linear, LayerNorm, SiLU twice, "
+                         "Linear, eps 1e-5); this block's has other layers")
     for tag, i_lin, i_ln in (("0", 0, 1), ("1", 3, 4)):
         inputs[f"rad_w{tag}"] = t(rad[i_lin].weight).unsqueeze(0)
         inputs[f"rad_b{tag}"] = t(rad[i_lin].bias).unsqueeze(0)
