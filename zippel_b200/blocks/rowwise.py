@@ -5,9 +5,11 @@
     dropout_add_layer_norm(x, residual, ...)         s = residual + dropout(x) and layer_norm(s), both
                                                      returned: the join of two layers of a residual network
 
-fp32, fp16 and bf16, any leading axes, any width of the last; rows of a wider array are read where they
-lie.  Sums and row statistics are fp32, each result is rounded once, and sums over rows (the gradients
-of weight and bias) are taken in a fixed order.  First order only, as every function of this package.
+fp32, fp16 and bf16, any leading axes, any width of the last; rows that lie one distance apart, a width at
+least, are read where they are, others (expanded or overlapping ones) from a copy.  Sums and row statistics
+are fp32, each result is rounded once, and sums over rows (the gradients of weight and bias) are taken in a
+fixed order.  First order only, as every function of this package.  Calls under ``torch.jit.trace`` and
+``make_fx`` are refused: they would leave a constant in the trace.
 
 Dropout stores no mask: which elements are kept follows from ``state``, two int64 on the device (seed and
 offset), and each element's number in the tensor, so the backward finds them again.  ``dropout_state``

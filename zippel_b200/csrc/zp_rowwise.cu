@@ -532,7 +532,6 @@ int zp_add_layernorm_backward(int64_t rows, int64_t width, int dtype, const void
   ZpNormCall c = {};
   c.rows = rows; c.width = width; c.x = sum; c.ldx = width; c.w = weight; c.mean_in = mean; c.rstd_in = rstd;
   c.dy = dy; c.ldy = ldy; c.dsum = dsum; c.lds = lds; c.dx = dx; c.dres = dresidual; c.dw = dweight; c.db = dbias;
- 
   cudaStream_t st = (cudaStream_t)stream;
   if (rows == 0) return p >= 0.0 && p <= 1.0 ? zero_params(c, param_dtype, st) : (int)ZP_ERR_INVALID_ARG;
   if (!make_drop(p, state, c.drop)) return ZP_ERR_INVALID_ARG;
