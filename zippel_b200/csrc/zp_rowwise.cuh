@@ -583,7 +583,7 @@ struct ZpTeamPlan {
   bool full, vectors;
   int slot, bytes, stages;                     // bytes of a slot, of the counters' bits of a team
   size_t smem;
-  ZpOver over;                                 // the width
+  ZpOver over;                                 // one over the width
   unsigned blocks;                             // 0 once a device has been found to run none of the plan's clusters
 };
 // The largest number of teams up to `most` of which every class of the cycle has as many

@@ -3,8 +3,8 @@
 //
 // Written against torch's C++ interface, unlike the rest of this package's binding, for the time of a call: a
 // layer norm of a few rows, forward and backward, takes 115 us with an autograd function in Python, of which
-// the kernels are 6, and the kernels of 16384 rows of 4096 are as long as that.  Here it is 63 to 66 (around torch's own layer
-// norm 68 to 71), and the forward alone 4 instead of 11.
+// the kernels are 6, and the kernels of 16384 rows of 4096 are as long as that.  Here it is 63 to 66 (around
+// torch's own layer norm 68 to 71), and the forward alone 4 instead of 11.
 #include <Python.h>
 
 #include <ATen/ATen.h>
